@@ -263,6 +263,69 @@ int occamy_noalloc_last_error(int clear);
 /* Bytes of the fixed array available to one call's working copies. */
 int64_t occamy_noalloc_capacity(void);
 
+/* ---- 8-bit and grouped products, expert layers ---------------------------------- */
+/* No counterpart in the reference: products whose operands are 8-bit numbers with a scale for each block, products of rows
+ * that go to different matrices, and what an expert layer needs around them.  Rules for all of them:
+ *   - tensors are row-major; `ld...` is the distance between rows, in elements.  Element types: 0 fp32, 1 bf16, 2 fp16,
+ *     3 e4m3 (8-bit floating point, largest value 448, no infinity).
+ *   - every pointer is memory of the CURRENT device, results overlap no input, and work is enqueued on `stream`, a stream of
+ *     that device; nothing waits and nothing is allocated, so calls can be captured into a graph.  `stream` may be any,
+ *     occamy_stream() among them.  Memory that came from wrapDNNMalloc or a pool is brought up to date first (a result
+ *     that a convolution left in another format, for instance) and ordered with the runtime's own stream on both sides;
+ *     while `stream` is captured such memory is refused (-6), unless `stream` is occamy_stream().
+ *   - results have the same bits from call to call; elements of a result's rows behind its columns, and rows
+ *     that no group or index reaches, are left as they were.  Sums are held in fp32.
+ *   - returns 0 (also for an empty problem, which launches nothing), a negative code with a line on stderr and nothing
+ *     enqueued (-1 no usable device, -2 workspace too small, -3 argument out of range, -5 a pointer that is not memory of the
+ *     current device, -6 as above), or a cudaError_t.  The products' kernels have bounded waits: one that ran out leaves garbage
+ *     in the result and a code that occamy_synchronize() collects for occamy_last_error(). */
+
+/* q = e4m3(x / s), s = 2^e with the smallest e >= -126 that keeps max|x| of the block within 448 s.  x has type 0, 1 or 2.
+ * blockRows 1: a block is 128 elements of a row, and row i of q is row index[i] of x (index null: row i, and rows == xRows);
+ * rows whose index is outside [0, xRows) are left as they were, their scales too.  blockRows 128: a block is 128 x 128.
+ * The last blocks may be smaller.  scales: [ceil(rows / blockRows)][ceil(cols / 128)], dense.  Infinities and NaN become NaN and
+ * do not count for the scale. */
+int occamy_quantize_e4m3(const void *x, int xType, int64_t xRows, int64_t cols, int64_t ldx,
+                         const int32_t *index, int64_t rows, int64_t blockRows, void *q, int64_t ldq,
+                         float *scales, cudaStream_t stream);
+/* out[M][N] = act(A B^T + bias) of e4m3 A[M][K] and B[N][K]: the value of A[m][k] is a * scaleA[m][k / 128], that of B[n][k]
+ * b * scaleB[n / 128][k / 128]; both scale arrays are dense, of any fp32 numbers.  bias [N] or null, fp32.  activMode as in
+ * DNNConvBiasActivFunc and DNNActiveFunc, 0 sigmoid, 1 ReLU, 2 tanh, 3 clip to [0, 6], 5 identity, and 6: x * sigmoid(x).
+ * outType 0, 1 or 2.  A and B start at multiples of 16 bytes, and so do their rows (lda % 16 == 0, ldb % 16 == 0). */
+int occamy_matmul_e4m3(const void *a, int64_t lda, const float *scaleA, const void *b, int64_t ldb,
+                       const float *scaleB, const float *bias, int64_t M, int64_t N, int64_t K,
+                       int64_t activMode, void *out, int outType, int64_t ldo, cudaStream_t stream);
+/* The same for rows in groups: rows offsets[g] .. offsets[g + 1] - 1 of out are the rows of A times matrix g of B.
+ * offsets: groups + 1 numbers in device memory, ascending, cut off at [0, rows]; rows in front of the first and behind the last are
+ * left as they were.  Row i is row index[i] of A[aRows][K], one outside [0, aRows) counts as zeros (index null: row i, and rows ==
+ * aRows).  type 1 or 2: A and B are bf16 / fp16 and have no scales; type 3: as above, with scaleB [groups][ceil(N / 128)]
+ * [ceil(K / 128)].  B: [groups][N][K], rows ldb apart, bias: [groups][N] or null.  Up to 1024 groups.
+ * activMode 7: out = silu(first) * second of two matrices for each group; then B is [groups][2][N][K], scaleB and bias have
+ * that 2 as well, and N % 8 == 0. */
+int occamy_matmul_grouped(const void *a, int type, int64_t aRows, int64_t lda, const float *scaleA,
+                          const int32_t *index, const int32_t *offsets, int64_t groups, const void *b,
+                          int64_t ldb, const float *scaleB, const float *bias, int64_t rows, int64_t N,
+                          int64_t K, int64_t activMode, void *out, int outType, int64_t ldo,
+                          cudaStream_t stream);
+/* The k largest logits of each token (type 0, 1 or 2; 1 to 1024 experts, k <= 32): chosen[tokens][k], largest first, ties to the
+ * lower expert, NaN above all; weights[tokens][k] their softmax, over all experts or (normalise != 0) over the chosen ones.
+ * An expert whose logit is -inf is never taken: such places have chosen -1, weight 0, position -1.  The taken (token, choice)
+ * pairs in the order of their expert, then token, then choice are the rows of the expert layer: offsets[experts + 1] where each
+ * expert's rows begin, order[tokens * k] the token of each row (-1 behind the last), position[tokens][k] the row of each pair.
+ * `order` and `offsets` are the index and offsets of the calls above.  The workspace is written by the call and may be used for
+ * anything after it; calls that can overlap on the GPU need one each. */
+int occamy_route_experts(const void *logits, int type, int64_t tokens, int64_t experts, int64_t ldl,
+                         int64_t k, int normalise, int32_t *chosen, float *weights, int32_t *offsets,
+                         int32_t *order, int32_t *position, void *workspace, int64_t workspaceBytes,
+                         cudaStream_t stream);
+/* Bytes of that workspace, or -3. */
+int64_t occamy_route_experts_workspace(int64_t tokens, int64_t experts, int64_t k);
+/* out[t] = sum over j of weights[t][j] * y[position[t][j]], in the order of j; places outside [0, yRows) count nothing.
+ * y [yRows][N] and out [tokens][N] have type 0, 1 or 2; k <= 32. */
+int occamy_combine_experts(const void *y, int type, int64_t yRows, int64_t ldy, const int32_t *position,
+                           const float *weights, int64_t tokens, int64_t k, int64_t N, void *out,
+                           int outType, int64_t ldo, cudaStream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -1,0 +1,320 @@
+// Entry points of the 8-bit and grouped operators: argument checks, the order between the caller's stream and the
+// runtime's, launches.
+#include <climits>
+#include <cstdarg>
+#include <mutex>
+
+#include "expert_ops.h"
+#include "graph_replay.h"
+#include "kernels.h"
+#include "runtime.h"
+
+extern "C" void occamy_internal_opaque_call(void);
+
+using namespace occ;
+
+namespace {
+
+constexpr int MAX_DEVICES = 64;
+constexpr int NO_DEVICE = -1, TOO_SMALL = -2, BAD_ARGUMENT = -3, FAILED = -4, BAD_POINTER = -5, CAPTURED = -6;
+constexpr int64_t MOST_EXPERTS = 1024, MOST_CHOICES = 32;
+
+// Calls may come from several host threads; what they share (the tensor registry, counters, first-use set-up) is
+// not made for that.
+std::mutex g_mutex;
+
+int refuse(int code, const char *who, const char *why, ...) {
+  char text[256];
+  va_list ap;
+  va_start(ap, why);
+  vsnprintf(text, sizeof(text), why, ap);
+  va_end(ap);
+  fprintf(stderr, "[occamy_b200] %s: %s\n", who, text);
+  return code;
+}
+
+// One call: the current device, the pointers it was given, and the runtime's own stream.
+//
+// Memory that the runtime knows (wrapDNNMalloc, a pool) may not hold yet what it stands for: a zero fill or an upload that
+// is put off, a result kept in another format, a convolution held back.  Such tensors are brought up to date first, on the
+// runtime's stream; the caller's stream waits for that, and the runtime's for the call.
+class Call {
+ public:
+  Call(const char *who, cudaStream_t stream) : who_(who), stream_(stream) {}
+
+  int open() {
+    if (cudaGetDevice(&device_) != cudaSuccess || device_ < 0 || device_ >= MAX_DEVICES)
+      return refuse(NO_DEVICE, who_, "no usable current device");
+    static int sms[MAX_DEVICES] = {};
+    if (!sms[device_]) {
+      int major = 0;
+      if (cudaDeviceGetAttribute(&major, cudaDevAttrComputeCapabilityMajor, device_) != cudaSuccess || major != 10)
+        return refuse(NO_DEVICE, who_, "device %d is not sm_100", device_);
+      if (cudaDeviceGetAttribute(&sms[device_], cudaDevAttrMultiProcessorCount, device_) != cudaSuccess)
+        return refuse(NO_DEVICE, who_, "cannot read the number of SMs");
+    }
+    num_sms_ = sms[device_];
+    if (stream_ == rt().stream) {
+      occamy_internal_opaque_call();
+      settled_ = true;
+    }
+    return 0;
+  }
+  // Device memory that the call reads / writes; null is passed over.  `align`: of the address, in bytes.
+  int in(const void *p, size_t align) { return use(p, align, false); }
+  int out(void *p, size_t align) { return use(p, align, true); }
+
+  // Before the launches.  Nothing has been enqueued on the caller's stream so far.
+  int begin() {
+    if (!tracked_ || stream_ == rt().stream) return 0;
+    return order(rt().stream, stream_);
+  }
+  // `e`: of the launches.
+  int end(cudaError_t e) {
+    if (e != cudaSuccess) {
+      cudaGetLastError();
+      return refuse((int)e, who_, "%s", cudaGetErrorString(e));
+    }
+    count(CNT_LAUNCHES, 1);
+    if (!tracked_ || stream_ == rt().stream) return 0;
+    return order(stream_, rt().stream);
+  }
+  int num_sms() const { return num_sms_; }
+  const char *who() const { return who_; }
+
+ private:
+  int use(const void *p, size_t align, bool written) {
+    if (!p) return 0;
+    if ((uintptr_t)p % align) return refuse(BAD_ARGUMENT, who_, "an address is not a multiple of %zu bytes", align);
+    cudaPointerAttributes at;
+    if (cudaPointerGetAttributes(&at, p) != cudaSuccess) {
+      cudaGetLastError();
+      return refuse(BAD_POINTER, who_, "an address is not known to CUDA");
+    }
+    if (at.type != cudaMemoryTypeManaged && (at.type != cudaMemoryTypeDevice || at.device != device_))
+      return refuse(BAD_POINTER, who_, "an address is not memory of the current device");
+    if (!reg_find(p)) return 0;
+    if (stream_ != rt().stream) {
+      cudaStreamCaptureStatus st = cudaStreamCaptureStatusNone;
+      if (cudaStreamIsCapturing(stream_, &st) != cudaSuccess || st != cudaStreamCaptureStatusNone) {
+        cudaGetLastError();
+        return refuse(CAPTURED, who_, "memory of the runtime's own cannot be used while the stream is captured");
+      }
+    }
+    if (!settled_) {
+      occamy_internal_opaque_call();
+      settled_ = true;
+    }
+    tracked_ = true;
+    ensure_f32(p);   // a result may leave parts of its memory as they were: they have to be there too
+    if (written) mark_f32(const_cast<void *>(p));
+    return 0;
+  }
+  int order(cudaStream_t first, cudaStream_t then) {
+    cudaEvent_t ev;
+    cudaError_t e = cudaEventCreateWithFlags(&ev, cudaEventDisableTiming);
+    if (e == cudaSuccess) {
+      e = cudaEventRecord(ev, first);
+      if (e == cudaSuccess) e = cudaStreamWaitEvent(then, ev, 0);
+      cudaEventDestroy(ev);
+    }
+    if (e == cudaSuccess) return 0;
+    cudaGetLastError();
+    return refuse((int)e, who_, "%s", cudaGetErrorString(e));
+  }
+
+  const char *who_;
+  cudaStream_t stream_;
+  int device_ = -1, num_sms_ = 0;
+  bool settled_ = false, tracked_ = false;
+};
+
+bool extent(int64_t v) { return v >= 0 && v <= INT_MAX; }
+bool real_type(int t) { return t == ELEM_F32 || t == ELEM_BF16 || t == ELEM_F16; }
+// Rows `ld` elements apart, `cols` of them used: within 40 bits of bytes, as the copy engine's strides are.
+bool row_length(int64_t ld, int64_t cols, int64_t rows, int size) {
+  return ld >= cols && ld <= INT64_MAX / 16 && ld * size < (1ll << 40) && (rows <= 1 || ld <= INT64_MAX / 16 / rows);
+}
+bool linear_act(int64_t mode) {
+  return mode == ACT_SIGMOID || mode == ACT_RELU || mode == ACT_TANH || mode == ACT_CLIP || mode == ACT_IDENTITY ||
+         mode == ACT_SILU;
+}
+
+#define TRY(expr)               \
+  do {                          \
+    if (int c_ = (expr)) return c_; \
+  } while (0)
+
+// The products' common part.  `rows`: of the result.
+int product(Call &call, ProductArgs &p, cudaStream_t stream) {
+  const char *who = call.who();
+  if (!extent(p.a_rows) || !extent(p.rows) || !extent(p.N) || !extent(p.groups) || p.K < 1 || p.K > INT_MAX)
+    return refuse(BAD_ARGUMENT, who, "extent out of range");
+  const int both = p.act == ACT_GATED_SILU ? 2 : 1, es = elem_size(p.type);
+  const int64_t mats = p.groups * both;
+  if (!real_type(p.out_type)) return refuse(BAD_ARGUMENT, who, "type of the result");
+  if (mats * p.N > INT_MAX) return refuse(BAD_ARGUMENT, who, "more than 2^31 - 1 rows of weights");
+  if (!row_length(p.lda, p.K, p.a_rows, es) || !row_length(p.ldb, p.K, mats * p.N, es) || !row_length(p.ldo, p.N, p.rows, 4))
+    return refuse(BAD_ARGUMENT, who, "distance between rows out of range");
+  if (p.lda * es % 16 || p.ldb * es % 16)
+    return refuse(BAD_ARGUMENT, who, "rows of the operands have to start at multiples of 16 bytes");
+  if (both == 2 && p.N % 8) return refuse(BAD_ARGUMENT, who, "a gated product needs N %% 8 == 0");
+  const bool scaled = p.type == ELEM_E4M3;
+  if (p.rows == 0 || p.N == 0) return 0;
+  if (p.a_rows == 0) return refuse(BAD_ARGUMENT, who, "A has no rows");
+  if (!p.a || !p.b || !p.out || (scaled && (!p.scale_a || !p.scale_b)))
+    return refuse(BAD_ARGUMENT, who, "null pointer");
+  if (!scaled) p.scale_a = p.scale_b = nullptr;
+  TRY(call.open());
+  TRY(call.in(p.a, 16));
+  TRY(call.in(p.b, 16));
+  TRY(call.in(p.scale_a, 4));
+  TRY(call.in(p.scale_b, 4));
+  TRY(call.in(p.bias, 4));
+  TRY(call.in(p.index, 4));
+  TRY(call.in(p.offsets, 4));
+  TRY(call.out(p.out, elem_size(p.out_type)));
+  p.err = rt().dev_err;
+  TRY(call.begin());
+  return call.end(launch_product(p, call.num_sms(), stream));
+}
+
+}  // namespace
+
+extern "C" {
+
+int occamy_quantize_e4m3(const void *x, int xType, int64_t xRows, int64_t cols, int64_t ldx, const int32_t *index,
+                         int64_t rows, int64_t blockRows, void *q, int64_t ldq, float *scales, cudaStream_t stream) try {
+  std::lock_guard<std::mutex> lock(g_mutex);
+  Call call("occamy_quantize_e4m3", stream);
+  if (!real_type(xType)) return refuse(BAD_ARGUMENT, call.who(), "type of x");
+  if (!extent(xRows) || !extent(cols) || !extent(rows)) return refuse(BAD_ARGUMENT, call.who(), "extent out of range");
+  if (blockRows != 1 && blockRows != SCALE_BLOCK) return refuse(BAD_ARGUMENT, call.who(), "blockRows is 1 or 128");
+  if (index && blockRows != 1) return refuse(BAD_ARGUMENT, call.who(), "an index needs blockRows 1");
+  if (!index && rows != xRows) return refuse(BAD_ARGUMENT, call.who(), "rows other than xRows need an index");
+  if (!row_length(ldx, cols, xRows, elem_size(xType)) || !row_length(ldq, cols, rows, 1))
+    return refuse(BAD_ARGUMENT, call.who(), "distance between rows out of range");
+  if (rows == 0 || cols == 0 || xRows == 0) return 0;
+  if (!x || !q || !scales) return refuse(BAD_ARGUMENT, call.who(), "null pointer");
+  TRY(call.open());
+  TRY(call.in(x, elem_size(xType)));
+  TRY(call.in(index, 4));
+  TRY(call.out(q, 1));
+  TRY(call.out(scales, 4));
+  TRY(call.begin());
+  QuantArgs a = {x, xType, xRows, cols, ldx, index, rows, (int)blockRows, (uint8_t *)q, ldq, scales};
+  return call.end(launch_quantize_e4m3(a, call.num_sms(), stream));
+} catch (...) {
+  return FAILED;
+}
+
+int occamy_matmul_e4m3(const void *a, int64_t lda, const float *scaleA, const void *b, int64_t ldb, const float *scaleB,
+                       const float *bias, int64_t M, int64_t N, int64_t K, int64_t activMode, void *out, int outType,
+                       int64_t ldo, cudaStream_t stream) try {
+  std::lock_guard<std::mutex> lock(g_mutex);
+  Call call("occamy_matmul_e4m3", stream);
+  if (!linear_act(activMode)) return refuse(BAD_ARGUMENT, call.who(), "activation mode (0, 1, 2, 3, 5 or 6)");
+  ProductArgs p = {};
+  p.a = a; p.b = b; p.type = ELEM_E4M3;
+  p.a_rows = p.rows = M; p.lda = lda; p.ldb = ldb;
+  p.scale_a = scaleA; p.scale_b = scaleB; p.bias = bias;
+  p.groups = 1; p.N = N; p.K = K;
+  p.act = (int)activMode; p.out = out; p.out_type = outType; p.ldo = ldo;
+  return product(call, p, stream);
+} catch (...) {
+  return FAILED;
+}
+
+int occamy_matmul_grouped(const void *a, int type, int64_t aRows, int64_t lda, const float *scaleA, const int32_t *index,
+                          const int32_t *offsets, int64_t groups, const void *b, int64_t ldb, const float *scaleB,
+                          const float *bias, int64_t rows, int64_t N, int64_t K, int64_t activMode, void *out,
+                          int outType, int64_t ldo, cudaStream_t stream) try {
+  std::lock_guard<std::mutex> lock(g_mutex);
+  Call call("occamy_matmul_grouped", stream);
+  if (type != ELEM_BF16 && type != ELEM_F16 && type != ELEM_E4M3)
+    return refuse(BAD_ARGUMENT, call.who(), "type of the operands");
+  if (!linear_act(activMode) && activMode != ACT_GATED_SILU)
+    return refuse(BAD_ARGUMENT, call.who(), "activation mode (0, 1, 2, 3, 5, 6 or 7)");
+  if (groups < 0 || groups > MOST_EXPERTS) return refuse(BAD_ARGUMENT, call.who(), "0 to 1024 groups");
+  if (!index && rows != aRows) return refuse(BAD_ARGUMENT, call.who(), "rows other than aRows need an index");
+  if (rows > 0 && groups > 0 && !offsets) return refuse(BAD_ARGUMENT, call.who(), "null pointer");
+  if (groups == 0) return 0;
+  ProductArgs p = {};
+  p.a = a; p.b = b; p.type = type;
+  p.a_rows = aRows; p.rows = rows; p.lda = lda; p.ldb = ldb;
+  p.scale_a = scaleA; p.scale_b = scaleB; p.bias = bias;
+  p.index = index; p.offsets = offsets; p.groups = groups; p.N = N; p.K = K;
+  p.act = (int)activMode; p.out = out; p.out_type = outType; p.ldo = ldo;
+  return product(call, p, stream);
+} catch (...) {
+  return FAILED;
+}
+
+int64_t occamy_route_experts_workspace(int64_t tokens, int64_t experts, int64_t k) {
+  if (!extent(tokens) || experts < 1 || experts > MOST_EXPERTS || k < 1 || k > MOST_CHOICES) return BAD_ARGUMENT;
+  return (int64_t)route_workspace(tokens, experts, k);
+}
+
+int occamy_route_experts(const void *logits, int type, int64_t tokens, int64_t experts, int64_t ldl, int64_t k,
+                         int normalise, int32_t *chosen, float *weights, int32_t *offsets, int32_t *order,
+                         int32_t *position, void *workspace, int64_t workspaceBytes, cudaStream_t stream) try {
+  std::lock_guard<std::mutex> lock(g_mutex);
+  Call call("occamy_route_experts", stream);
+  if (!real_type(type)) return refuse(BAD_ARGUMENT, call.who(), "type of the logits");
+  if (!extent(tokens)) return refuse(BAD_ARGUMENT, call.who(), "extent out of range");
+  if (experts < 1 || experts > MOST_EXPERTS) return refuse(BAD_ARGUMENT, call.who(), "1 to 1024 experts");
+  if (k < 1 || k > MOST_CHOICES || k > experts)
+    return refuse(BAD_ARGUMENT, call.who(), "1 to 32 choices, no more than experts");
+  if (tokens * k > INT_MAX) return refuse(BAD_ARGUMENT, call.who(), "more than 2^31 - 1 rows");
+  if (!row_length(ldl, experts, tokens, elem_size(type)))
+    return refuse(BAD_ARGUMENT, call.who(), "distance between rows out of range");
+  if (!offsets || (tokens && (!logits || !chosen || !weights || !order || !position)))
+    return refuse(BAD_ARGUMENT, call.who(), "null pointer");
+  const size_t need = route_workspace(tokens, experts, k);
+  if (need && (!workspace || workspaceBytes < (int64_t)need))
+    return refuse(TOO_SMALL, call.who(), "the workspace has to have %zu bytes", need);
+  TRY(call.open());
+  TRY(call.out(offsets, 4));
+  if (tokens == 0) {
+    TRY(call.begin());
+    return call.end(cudaMemsetAsync(offsets, 0, (size_t)(experts + 1) * 4, stream));
+  }
+  TRY(call.in(logits, elem_size(type)));
+  TRY(call.out(chosen, 4));
+  TRY(call.out(weights, 4));
+  TRY(call.out(order, 4));
+  TRY(call.out(position, 4));
+  TRY(call.out(workspace, 4));
+  TRY(call.begin());
+  RouteArgs a = {logits, type, tokens, experts, ldl, (int)k, normalise != 0, chosen, weights, offsets, order, position,
+                 (int32_t *)workspace};
+  return call.end(launch_route(a, stream));
+} catch (...) {
+  return FAILED;
+}
+
+int occamy_combine_experts(const void *y, int type, int64_t yRows, int64_t ldy, const int32_t *position,
+                           const float *weights, int64_t tokens, int64_t k, int64_t N, void *out, int outType,
+                           int64_t ldo, cudaStream_t stream) try {
+  std::lock_guard<std::mutex> lock(g_mutex);
+  Call call("occamy_combine_experts", stream);
+  if (!real_type(type) || !real_type(outType)) return refuse(BAD_ARGUMENT, call.who(), "element type");
+  if (!extent(yRows) || !extent(tokens) || !extent(N)) return refuse(BAD_ARGUMENT, call.who(), "extent out of range");
+  if (k < 1 || k > MOST_CHOICES) return refuse(BAD_ARGUMENT, call.who(), "1 to 32 choices");
+  if (!row_length(ldy, N, yRows, elem_size(type)) || !row_length(ldo, N, tokens, elem_size(outType)))
+    return refuse(BAD_ARGUMENT, call.who(), "distance between rows out of range");
+  if (tokens == 0 || N == 0) return 0;
+  if ((yRows && !y) || !position || !weights || !out) return refuse(BAD_ARGUMENT, call.who(), "null pointer");
+  TRY(call.open());
+  if (yRows) TRY(call.in(y, elem_size(type)));
+  TRY(call.in(position, 4));
+  TRY(call.in(weights, 4));
+  TRY(call.out(out, elem_size(outType)));
+  TRY(call.begin());
+  CombineArgs a = {y, type, yRows, ldy, position, weights, tokens, k, N, out, outType, ldo};
+  return call.end(launch_combine(a, call.num_sms(), stream));
+} catch (...) {
+  return FAILED;
+}
+
+}  // extern "C"

@@ -89,6 +89,20 @@ _SIGNATURES = {
                                                C.c_int64, _f32p, C.c_void_p]),
     "occamy_noalloc_last_error": (C.c_int, [C.c_int]),
     "occamy_noalloc_capacity": (C.c_int64, []),
+    "occamy_quantize_e4m3": (C.c_int, [C.c_void_p, C.c_int, C.c_int64, C.c_int64, C.c_int64, C.c_void_p, C.c_int64,
+                                       C.c_int64, C.c_void_p, C.c_int64, C.c_void_p, C.c_void_p]),
+    "occamy_matmul_e4m3": (C.c_int, [C.c_void_p, C.c_int64, C.c_void_p, C.c_void_p, C.c_int64, C.c_void_p, C.c_void_p,
+                                     C.c_int64, C.c_int64, C.c_int64, C.c_int64, C.c_void_p, C.c_int, C.c_int64,
+                                     C.c_void_p]),
+    "occamy_matmul_grouped": (C.c_int, [C.c_void_p, C.c_int, C.c_int64, C.c_int64, C.c_void_p, C.c_void_p, C.c_void_p,
+                                        C.c_int64, C.c_void_p, C.c_int64, C.c_void_p, C.c_void_p, C.c_int64, C.c_int64,
+                                        C.c_int64, C.c_int64, C.c_void_p, C.c_int, C.c_int64, C.c_void_p]),
+    "occamy_route_experts": (C.c_int, [C.c_void_p, C.c_int, C.c_int64, C.c_int64, C.c_int64, C.c_int64, C.c_int,
+                                       C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p,
+                                       C.c_int64, C.c_void_p]),
+    "occamy_route_experts_workspace": (C.c_int64, [C.c_int64, C.c_int64, C.c_int64]),
+    "occamy_combine_experts": (C.c_int, [C.c_void_p, C.c_int, C.c_int64, C.c_int64, C.c_void_p, C.c_void_p, C.c_int64,
+                                         C.c_int64, C.c_int64, C.c_void_p, C.c_int, C.c_int64, C.c_void_p]),
     "occamy_fused_chains": (C.c_int64, []),
     "occamy_set_cross_call_fusion": (None, [C.c_int]),
     "occamy_profile_begin": (None, []),
@@ -101,6 +115,9 @@ for _r in (2, 3, 4, 6):
                                                                 _i64p, _i64p, C.c_int64])
 
 MATH_FP32, MATH_BF16, MATH_F16 = 0, 1, 2
+# element types of the 8-bit and grouped operators, and their activations beyond the reference's
+F32, BF16, F16, E4M3 = 0, 1, 2, 3
+ACT_SILU, ACT_GATED_SILU = 6, 7
 COUNTER_NAMES = ("launches", "h2d_bytes", "h2d_skipped_bytes", "pool_hwm_bytes", "tc_launches",
                  "materializations", "tmap_encodes", "simt_launches")
 
