@@ -495,7 +495,7 @@ TcFastDiv make_fastdiv(int d) {
 
 #ifdef OCCAMY_TC_TIMERS
 // analysis builds only: the device words the kernels' role timers add to
-static long long *tc_timer_words() {
+long long *tc_timer_words() {
   static long long *w = nullptr;
   if (!w) {
     cudaMalloc(&w, 20 * sizeof(long long));

@@ -75,19 +75,27 @@ cudaError_t launch_route(const RouteArgs &a, cudaStream_t s);
 size_t route_workspace(int64_t tokens, int64_t experts, int64_t k);
 cudaError_t launch_combine(const CombineArgs &a, int num_sms, cudaStream_t s);
 
-// A launch that may start while the kernel before it is still running: the kernel begins with chain_begin().
+#ifdef OCCAMY_TC_TIMERS
+long long *tc_timer_words();   // conv_tc.cu
+#endif
+
+// A launch that may start while the kernel before it is still running: the kernel begins with chain_begin().  `cluster`: CTAs
+// that run together.
 template <typename... P, typename... A>
-inline cudaError_t launch_after(void (*kernel)(P...), dim3 grid, dim3 block, size_t smem, cudaStream_t s, A... args) {
+inline cudaError_t launch_after(void (*kernel)(P...), dim3 grid, dim3 block, size_t smem, cudaStream_t s, int cluster, A... args) {
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = grid;
   cfg.blockDim = block;
   cfg.dynamicSmemBytes = smem;
   cfg.stream = s;
-  cudaLaunchAttribute attr;
-  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr.val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = &attr;
-  cfg.numAttrs = 1;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = (unsigned)cluster;
+  attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = cluster > 1 ? 2 : 1;
   return cudaLaunchKernelEx(&cfg, kernel, static_cast<P>(args)...);
 }
 

@@ -183,7 +183,7 @@ __global__ void __launch_bounds__(RT_THREADS) route_place_kernel(RouteArgs a, in
 
 template <int V>
 cudaError_t launch_choose(const RouteArgs &a, unsigned blocks, int64_t per_block, cudaStream_t s) {
-  return launch_after(route_choose_kernel<V>, dim3(blocks), dim3(RT_THREADS), (size_t)a.experts * 4, s, a, per_block);
+  return launch_after(route_choose_kernel<V>, dim3(blocks), dim3(RT_THREADS), (size_t)a.experts * 4, s, 1, a, per_block);
 }
 
 // ---------------------------------------------------------------- weighted sum
@@ -221,12 +221,12 @@ cudaError_t launch_route(const RouteArgs &a, cudaStream_t s) {
   else e = launch_choose<32>(a, blocks, per, s);
   if (e != cudaSuccess) return e;
   const size_t smem = (size_t)a.experts * 4 * (2 + place_warps(a.experts));
-  return launch_after(route_place_kernel, dim3(blocks), dim3(RT_THREADS), smem, s, a, per);
+  return launch_after(route_place_kernel, dim3(blocks), dim3(RT_THREADS), smem, s, 1, a, per);
 }
 
 cudaError_t launch_combine(const CombineArgs &a, int num_sms, cudaStream_t s) {
   const int64_t want = (a.tokens * a.N + 255) / 256, most = (int64_t)num_sms * 32;
-  return launch_after(combine_kernel, dim3((unsigned)(want < most ? want : most)), dim3(256), 0, s, a);
+  return launch_after(combine_kernel, dim3((unsigned)(want < most ? want : most)), dim3(256), 0, s, 1, a);
 }
 
 }  // namespace occ

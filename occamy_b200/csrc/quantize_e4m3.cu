@@ -107,11 +107,11 @@ cudaError_t launch_typed(const QuantArgs &a, int num_sms, cudaStream_t s) {
   const int64_t blocks = scale_blocks(a.cols);
   if (a.block_rows == 1) {
     const int64_t total = a.rows * blocks, want = (total + 7) / 8, most = (int64_t)num_sms * 32;
-    return launch_after(quantize_rows_kernel<T>, dim3((unsigned)(want < most ? want : most)), dim3(256), 0, s, a, blocks,
+    return launch_after(quantize_rows_kernel<T>, dim3((unsigned)(want < most ? want : most)), dim3(256), 0, s, 1, a, blocks,
                         total);
   }
   const int64_t total = scale_blocks(a.rows) * blocks, most = (int64_t)num_sms * 32;
-  return launch_after(quantize_blocks_kernel<T>, dim3((unsigned)(total < most ? total : most)), dim3(256), 0, s, a,
+  return launch_after(quantize_blocks_kernel<T>, dim3((unsigned)(total < most ? total : most)), dim3(256), 0, s, 1, a,
                       blocks, total);
 }
 
