@@ -298,7 +298,7 @@ int occamy_matmul_e4m3(const void *a, int64_t lda, const float *scaleA, const vo
 /* The same for rows in groups: rows offsets[g] .. offsets[g + 1] - 1 of out are the rows of A times matrix g of B.
  * offsets: groups + 1 numbers in device memory, ascending, cut off at [0, rows]; rows in front of the first and behind the last are
  * left as they were.  Row i is row index[i] of A[aRows][K], one outside [0, aRows) counts as zeros (index null: row i, and rows ==
- * aRows).  type 1 or 2: A and B are bf16 / fp16 and have no scales; type 3: as above, with scaleB [groups][ceil(N / 128)]
+ * aRows; with one, A has at most 64 GiB).  type 1 or 2: A and B are bf16 / fp16 and have no scales; type 3: as above, with scaleB [groups][ceil(N / 128)]
  * [ceil(K / 128)].  B: [groups][N][K], rows ldb apart, bias: [groups][N] or null.  Up to 1024 groups.
  * activMode 7: out = silu(first) * second of two matrices for each group; then B is [groups][2][N][K], scaleB and bias have
  * that 2 as well, and N % 8 == 0. */

@@ -25,10 +25,6 @@
 namespace occ {
 namespace {
 
-// Loads, MMAs, two warps of scales; then epilogue warps: four for each 32 or 64 columns, so that enough of them wait for TMEM
-// while others add, eight in narrow tiles.
-__host__ __device__ constexpr int pt_epi_warps(int bn) { return bn >= 128 ? 16 : 8; }
-__host__ __device__ constexpr int pt_threads(int bn) { return 128 + 32 * pt_epi_warps(bn); }
 constexpr int PT_ROWS = 128;           // weights of a tile
 constexpr int PT_PER = 4;              // k-steps of 16-bit operands that the tensor core adds up by itself
 
@@ -39,8 +35,8 @@ __device__ __forceinline__ float ld_cluster_f32(uint32_t addr) {
 }
 
 template <int BN, bool SCALED, bool GATED>
-__global__ void __launch_bounds__(pt_threads(BN), BN <= 64 ? 2 : 1) block_product_kernel(const __grid_constant__ PtParams p) {
-  constexpr int EW = pt_epi_warps(BN), THREADS = pt_threads(BN);
+__global__ void __launch_bounds__(PT_THREADS, BN <= 64 ? 2 : 1) block_product_kernel(const __grid_constant__ PtParams p) {
+  constexpr int EW = PT_EPI_WARPS;
   constexpr int CW = BN / (EW / 4);      // columns of an epilogue warp
   constexpr int NG = CW / 8;             // groups of eight of them
   constexpr int LD = CW < 32 ? CW : 32;  // columns of one TMEM load
@@ -72,10 +68,10 @@ __global__ void __launch_bounds__(pt_threads(BN), BN <= 64 ? 2 : 1) block_produc
   const int warp = warp_index(), lane = threadIdx.x & 31;
   constexpr uint32_t COLS = BN >= 128 ? 512 : BN * 4;
   if (threadIdx.x == 0) {
-    tma_prefetch_map(&p.ta);
+    if (!p.index) tma_prefetch_map(&p.ta);
     tma_prefetch_map(&p.tb);
     for (int s = 0; s < stages; ++s) {
-      mbar_init(full_bar(s), 1);
+      mbar_init(full_bar(s), p.index ? 1 + 32 * PT_GATHERERS : 1);   // loads, lanes that copy rows chosen by an index
       mbar_init(empty_bar(s), 1);
     }
     for (int b = 0; b < bufs; ++b) {
@@ -95,7 +91,7 @@ __global__ void __launch_bounds__(pt_threads(BN), BN <= 64 ? 2 : 1) block_produc
   }
   pdl_launch_dependents();
   pdl_wait();
-  pt_read_groups<THREADS>(p, groups);
+  pt_read_groups<PT_THREADS>(p, groups);
   __syncthreads();
   if (warp == 0) pt_count_tiles<BN>(p, groups, lane);
   tc_fence_before();
@@ -111,9 +107,8 @@ __global__ void __launch_bounds__(pt_threads(BN), BN <= 64 ? 2 : 1) block_produc
   int err_code = 0;
   auto decode = [&](int tile) { return pt_decode<BN, TILE_N>(p, groups, tile); };
 
-  // An epilogue warp's place; sums of weight `lane` of its quadrant and columns c0 + 2 i, 2 i + 1.
-  const int ew = warp - 4, quad = warp & 3, c0 = (ew >> 2) * CW;
-  uint64_t acc[CW / 2];
+  // An epilogue warp's place.
+  const int ew = warp - PT_EPI_WARP, quad = warp & 3, c0 = (ew >> 2) * CW;
 
   // Eight rows of results (columns c0 + 8 g ...) through 1 KB of shared memory, [row][32 weights].  There is one copy of the
   // code behind it: with the activations of all sums unrolled, fetching instructions took 30 us a tile.
@@ -159,6 +154,12 @@ __global__ void __launch_bounds__(pt_threads(BN), BN <= 64 ? 2 : 1) block_produc
                  n_tile - n_lane);
   };
 
+  // The sums' warps take the registers that the others do without: (256 x 48 + 256 x 208) = 512 x 128, of two CTAs (256 x 40 + 256 x
+  // 88) = 512 x 64.  (Each at the head of its roles: behind a point where both come together the compiler keeps to the smaller
+  // number.)
+  if (warp < PT_EPI_WARP) {
+  if constexpr (BN <= 64) asm volatile("setmaxnreg.dec.sync.aligned.u32 40;");
+  else asm volatile("setmaxnreg.dec.sync.aligned.u32 48;");
   if (warp == 0) {
     // ------------------------------------------------------------ loads
     TCT_DECL
@@ -166,14 +167,8 @@ __global__ void __launch_bounds__(pt_threads(BN), BN <= 64 ? 2 : 1) block_produc
     uint32_t phase = 0;
     for (int tile = tile0; tile < total && !err_code; tile += tstep) {
       const PtTile tl = decode(tile);
-      int4 rows4[BN > 128 ? 2 : 1];
-      const int n4 = (tl.rows + 3) / 4;
-      if (p.index) {
-#pragma unroll
-        for (int i = 0; i < (BN > 128 ? 2 : 1); ++i) rows4[i] = four_rows(p, tl.m0, tl.rows, lane + 32 * i);
-      }
-      const int boxes = (tl.rows + PT_BOX - 1) / PT_BOX;
-      const uint32_t bytes = W_BYTES + (p.index ? (uint32_t)n4 * 512u : (uint32_t)boxes * (PT_BOX * 128u));
+      const int boxes = p.index ? 0 : (tl.rows + PT_BOX - 1) / PT_BOX;
+      const uint32_t bytes = W_BYTES + (uint32_t)boxes * (PT_BOX * 128u);
       for (int kb = k0; kb < k1; ++kb) {
         if (!TCT_WAIT(0, mbar_wait_warp(empty_bar(stage), phase ^ 1u, abort_flag))) {
           err_code = 1;
@@ -181,19 +176,11 @@ __global__ void __launch_bounds__(pt_threads(BN), BN <= 64 ? 2 : 1) block_produc
         }
         const int k = kb * (SCALED ? 128 : 64);
         expect_tx_warp(full_bar(stage), bytes);
-        if constexpr (GATED) load_5d_warp<false>(sW + stage * W_BYTES, &p.tb, full_bar(stage), k, tl.n0 / 8, tl.g);
-        else load_2d_warp<false>(sW + stage * W_BYTES, &p.tb, full_bar(stage), k, tl.g * p.N + tl.n0);
+        if constexpr (GATED) load_5d_warp(sW + stage * W_BYTES, &p.tb, full_bar(stage), k, tl.n0 / 8, tl.g);
+        else load_2d_warp(sW + stage * W_BYTES, &p.tb, full_bar(stage), k, tl.g * p.N + tl.n0);
         const uint32_t dst = sR + stage * R_BYTES;
-        if (p.index) {
-#pragma unroll
-          for (int i = 0; i < (BN > 128 ? 2 : 1); ++i)
-            if (lane + 32 * i < n4)
-              gather_4_rows<false>(dst + (lane + 32 * i) * 512u, &p.ta, full_bar(stage), k, rows4[i]);
-          __syncwarp();
-        } else {
-          for (int b = 0; b < boxes; ++b)
-            load_2d_warp<false>(dst + b * (PT_BOX * 128u), &p.ta, full_bar(stage), k, tl.m0 + b * PT_BOX);
-        }
+        for (int b = 0; b < boxes; ++b)
+          load_2d_warp(dst + b * (PT_BOX * 128u), &p.ta, full_bar(stage), k, tl.m0 + b * PT_BOX);
         if (++stage == stages) {
           stage = 0;
           phase ^= 1u;
@@ -228,12 +215,13 @@ __global__ void __launch_bounds__(pt_threads(BN), BN <= 64 ? 2 : 1) block_produc
           err_code = 3;
           break;
         }
+        if (p.index) fence_async_smem();
         tc_fence_after();
         const uint32_t d = tmem + (uint32_t)(buf * BN);
         const uint32_t a = w_lo + (uint32_t)stage * (W_BYTES >> 4), b = r_lo + (uint32_t)stage * (R_BYTES >> 4);
 #pragma unroll
         for (int kk = 0; kk < 4; ++kk)
-          pt_mma<SCALED, false>(d, a + 2u * kk, hi, b + 2u * kk, hi, idesc, kk ? 1u : (uint32_t)(in_chunk != 0));
+          pt_mma<SCALED>(d, a + 2u * kk, hi, b + 2u * kk, hi, idesc, kk ? 1u : (uint32_t)(in_chunk != 0));
         commit_warp(empty_bar(stage));
         if (++stage == stages) {
           stage = 0;
@@ -250,12 +238,17 @@ __global__ void __launch_bounds__(pt_threads(BN), BN <= 64 ? 2 : 1) block_produc
       }
     }
     TCT_FLUSH(1)
-  } else if (warp < 4) {
+  } else if (warp >= PT_GATHER_WARP) {
+    // ------------------------------------------------------------ rows chosen by an index
+    if (p.index)
+      err_code = pt_gather_role<BN, PT_GATHERERS>(p, tile0, total, tstep, k0, k1, sR, stages, warp - PT_GATHER_WARP, lane, abort_flag,
+                                                  decode, full_bar, empty_bar);
+  } else {
     // ------------------------------------------------------------ scales
     // sA * sB of every column, one k-step after another.
     if constexpr (SCALED) {
       TCT_DECL
-      constexpr int MINE = (BN + 63) / 64;
+      constexpr int MINE = BN <= 64 ? 1 : BN / 64;
       const int t = threadIdx.x - 64;
       int buf = 0;
       uint32_t buf_phase = 0;
@@ -282,14 +275,6 @@ __global__ void __launch_bounds__(pt_threads(BN), BN <= 64 ? 2 : 1) block_produc
         };
         fetch(k0);
         for (int kq = k0; kq < k1 && !err_code; kq += 4) {
-          float w[4][SETS][MINE];
-#pragma unroll
-          for (int j = 0; j < 4; ++j)
-#pragma unroll
-            for (int h = 0; h < SETS; ++h)
-#pragma unroll
-              for (int i = 0; i < MINE; ++i) w[j][h][i] = va[i][j] * vb[h][j];
-          if (kq + 4 < k1) fetch(kq + 4);   // under way while these are waited for and written
 #pragma unroll
           for (int j = 0; j < 4; ++j) {
             if (kq + j >= k1 || err_code) continue;
@@ -297,12 +282,12 @@ __global__ void __launch_bounds__(pt_threads(BN), BN <= 64 ? 2 : 1) block_produc
               err_code = 4;
               continue;
             }
-            float *dst = scales + buf * (SETS * BN);
+            float *dst = scales + buf * (SETS * BN) + t;
 #pragma unroll
             for (int i = 0; i < MINE; ++i)
 #pragma unroll
               for (int h = 0; h < SETS; ++h)
-                if (BN >= 64 || t + 64 * i < BN) dst[h * BN + t + 64 * i] = w[j][h][i];
+                if (BN >= 64 || t < BN) dst[h * BN + 64 * i] = va[i][j] * vb[h][j];
             __syncwarp();
             if (lane == 0) mbar_arrive(sfull_bar(buf));
             if (++buf == bufs) {
@@ -310,13 +295,22 @@ __global__ void __launch_bounds__(pt_threads(BN), BN <= 64 ? 2 : 1) block_produc
               buf_phase ^= 1u;
             }
           }
+          if (kq + 4 < k1) fetch(kq + 4);
         }
       }
       if (warp == 2) { TCT_FLUSH(2) }
     }
+  }
+  if (splits > 1) {   // where the sums' warps meet, the CTAs of the cluster among them
+    __syncwarp();
+    cluster_sync_all();
+  }
   } else {
     // ------------------------------------------------------------ sums and results
+    if constexpr (BN <= 64) asm volatile("setmaxnreg.inc.sync.aligned.u32 88;");
+    else asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
     TCT_DECL
+    uint64_t acc[CW / 2];                  // sums of weight `lane` of the quadrant and columns c0 + 2 i, 2 i + 1
     int buf = 0;
     uint32_t buf_phase = 0;
     for (int tile = tile0; tile < total && !err_code; tile += tstep) {
@@ -368,6 +362,49 @@ __global__ void __launch_bounds__(pt_threads(BN), BN <= 64 ? 2 : 1) block_produc
         }
       }
       if (splits > 1 || err_code) break;
+      if (p.vec_out && (GATED || p.act == ACT_IDENTITY || p.act == ACT_RELU) && (tl.n0 + TILE_N <= p.N || p.N % 8 == 0)) {
+        // straight through all sums: a loop over them, as below, waits for one group's stores after another's loads
+        uint8_t *out = (uint8_t *)p.out + ((int64_t)(tl.m0 + c0 + row) * p.ldo + tl.n0 + n_lane) * (p.out_type == ELEM_F32 ? 4 : 2);
+        const int64_t step = p.ldo * (p.out_type == ELEM_F32 ? 32 : 16);
+        const bool here = tl.n0 + n_lane < p.N;
+        const float floor = !GATED && p.act == ACT_RELU ? 0.0f : -INFINITY;
+        float bias[8] = {};                // of this lane's weights
+        if (p.bias && here) {
+          const float *from = p.bias + (int64_t)tl.g * SETS * p.N + tl.n0 + n_lane;
+#pragma unroll
+          for (int j = 0; j < 8; ++j) bias[j] = __ldg(from + (GATED && j >= 4 ? p.N + j - 4 : j));
+        }
+#pragma unroll
+        for (int g = 0; g < NG; ++g, out += step) {
+          if (c0 + g * 8 >= tl.rows) break;
+          __syncwarp();
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            float a, b;
+            f2_unpack(acc[g * 4 + j], a, b);
+            buf_out[(2 * j) * 32 + lane] = a;
+            buf_out[(2 * j + 1) * 32 + lane] = b;
+          }
+          __syncwarp();
+          const float *src = buf_out + row * 32 + (GATED ? (piece >> 1) * 16 + (piece & 1) * 4 : piece * 8);
+          const float4 a = *reinterpret_cast<const float4 *>(src), b = *reinterpret_cast<const float4 *>(src + (GATED ? 8 : 4));
+          if (c0 + g * 8 + row < tl.rows && here) {
+            float r[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
+#pragma unroll
+            for (int j = 0; j < 8; ++j) r[j] += bias[j];
+            if constexpr (GATED) {
+#pragma unroll
+              for (int j = 0; j < 4; ++j) r[j] = silu(r[j]) * r[4 + j];
+              store_row<4, true>(p, out, r, 4);
+            } else {
+#pragma unroll
+              for (int j = 0; j < 8; ++j) asm("max.NaN.f32 %0, %0, %1;" : "+f"(r[j]) : "f"(floor));
+              store_row<8, true>(p, out, r, 8);
+            }
+          }
+        }
+        continue;
+      }
 #pragma unroll 1
       for (int g = 0; g < NG && c0 + g * 8 < tl.rows; ++g)
         finish(tl, g, [&](int g, auto &&put) {
@@ -383,38 +420,38 @@ __global__ void __launch_bounds__(pt_threads(BN), BN <= 64 ? 2 : 1) block_produc
         });
     }
     if (ew == 0 || ew == EW - 1) { TCT_FLUSH(ew ? 4 : 3) }
-  }
-  if (splits > 1) {
-    // Every copy has landed and every MMA of the tile is complete: the ring holds the sums now, [column pair][thread].
-    const bool mine = tile0 < total;
-    if (warp >= 4 && mine && !err_code) {
-      uint64_t *sums = reinterpret_cast<uint64_t *>(smem_raw);
+    if (splits > 1) {
+      // Every copy has landed and every MMA of the tile is complete: the ring holds the sums now, [column pair][thread].
+      const bool mine = tile0 < total && !err_code;
+      if (mine) {
+        uint64_t *sums = reinterpret_cast<uint64_t *>(smem_raw);
 #pragma unroll
-      for (int i = 0; i < CW / 2; ++i) sums[i * (EW * 32) + threadIdx.x - 128] = acc[i];
-    }
-    __syncwarp();
-    cluster_sync_all();
-    if (warp >= 4 && mine && !err_code) {
-      const PtTile tl = decode(tile0);
-#pragma unroll 1
-      for (int g = 0; g < NG && c0 + g * 8 < tl.rows; ++g) {
-        if ((ew * NG + g) % splits != rank) continue;
-        float t[8] = {};
-        for (int r = 0; r < splits; ++r) {
-          const uint32_t from = cluster_map(sW, (uint32_t)r) + (uint32_t)(g * 4 * EW * 32 + (int)threadIdx.x - 128) * 8u;
-#pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            t[2 * j] += ld_cluster_f32(from + j * (EW * 32 * 8));
-            t[2 * j + 1] += ld_cluster_f32(from + j * (EW * 32 * 8) + 4);
-          }
-        }
-        finish(tl, g, [&](int, auto &&put) {
-#pragma unroll
-          for (int j = 0; j < 4; ++j) put(j, t[2 * j], t[2 * j + 1]);
-        });
+        for (int i = 0; i < CW / 2; ++i) sums[i * (EW * 32) + threadIdx.x - 32 * PT_EPI_WARP] = acc[i];
       }
+      __syncwarp();
+      cluster_sync_all();
+      if (mine) {
+        const PtTile tl = decode(tile0);
+#pragma unroll 1
+        for (int g = 0; g < NG && c0 + g * 8 < tl.rows; ++g) {
+          if ((ew * NG + g) % splits != rank) continue;
+          float t[8] = {};
+          for (int r = 0; r < splits; ++r) {
+            const uint32_t from = cluster_map(sW, (uint32_t)r) + (uint32_t)(g * 4 * EW * 32 + (int)threadIdx.x - 32 * PT_EPI_WARP) * 8u;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+              t[2 * j] += ld_cluster_f32(from + j * (EW * 32 * 8));
+              t[2 * j + 1] += ld_cluster_f32(from + j * (EW * 32 * 8) + 4);
+            }
+          }
+          finish(tl, g, [&](int, auto &&put) {
+#pragma unroll
+            for (int j = 0; j < 4; ++j) put(j, t[2 * j], t[2 * j + 1]);
+          });
+        }
+      }
+      __syncwarp();
     }
-    __syncwarp();
   }
   if (err_code) {
     *abort_flag = 1;
@@ -452,7 +489,7 @@ bool encode(CUtensorMap *m, int type, const void *ptr, int rank, const cuuint64_
 template <int BN, bool SCALED, bool GATED>
 cudaError_t launch_tiles(PtParams &p, int64_t most_tiles, int num_sms, cudaStream_t s) {
   constexpr size_t LIMIT = BN <= 64 ? TC_SMEM_DUO : TC_SMEM_LIMIT;
-  constexpr int EW = pt_epi_warps(BN);
+  constexpr int EW = PT_EPI_WARPS;
   p.bufs = BN == 256 ? 2 : 4;
   const size_t misc = EW * 1024 + (SCALED ? p.bufs * (GATED ? 2 : 1) * BN * 4 : 0) + 8 * 3 * 4 + 16 +
                       (3 * (size_t)p.groups + 1) * 4;
@@ -472,7 +509,7 @@ cudaError_t launch_tiles(PtParams &p, int64_t most_tiles, int num_sms, cudaStrea
   if constexpr (BN <= 128)
     while (p.splits < 8 && most_tiles * p.splits * 2 <= resident && p.kblocks >= p.splits * 8) p.splits *= 2;
   const int64_t grid = p.splits > 1 ? most_tiles * p.splits : std::min<int64_t>(most_tiles, resident);
-  return launch_after(block_product_kernel<BN, SCALED, GATED>, dim3((unsigned)grid), dim3(pt_threads(BN)), smem, s,
+  return launch_after(block_product_kernel<BN, SCALED, GATED>, dim3((unsigned)grid), dim3(PT_THREADS), smem, s,
                       p.splits, p);
 }
 
@@ -495,16 +532,15 @@ cudaError_t launch_product(const ProductArgs &a, int num_sms, cudaStream_t s) {
   const int es = elem_size(a.type), bk = 128 / es;
   const int64_t each = (a.rows + a.groups - 1) / a.groups;
   const bool wide = scaled && each > 128;
-  bool pair = false;
-#ifdef OCCAMY_TUNING
-  if (const char *e = getenv("OCCAMY_PT_PAIR")) pair = wide && atoi(e);
-#endif
-  {
+  p.a = (const uint8_t *)a.a;
+  p.a_ld16 = (uint32_t)(a.lda * es / 16);
+  p.k_bytes = (int)(a.K * es);
+  if (!a.index) {
     const cuuint64_t dims[2] = {(cuuint64_t)a.K, (cuuint64_t)a.a_rows}, strides[1] = {(cuuint64_t)a.lda * es};
-    const cuuint32_t box[2] = {(cuuint32_t)bk, a.index ? 1u : (cuuint32_t)PT_BOX};
+    const cuuint32_t box[2] = {(cuuint32_t)bk, (cuuint32_t)PT_BOX};
     if (!encode(&p.ta, a.type, a.a, 2, dims, strides, box)) return cudaErrorInvalidValue;
   }
-  const cuuint32_t weights = wide && !pair ? 256 : 128;   // of one copy
+  const cuuint32_t weights = wide ? 256 : 128;   // of one copy
   if (gated) {
     // eight rows of the first matrix, the same eight of the second, and so on: both halves of a result are near each other
     const cuuint64_t ld = (cuuint64_t)a.ldb * es;
@@ -532,19 +568,19 @@ cudaError_t launch_product(const ProductArgs &a, int num_sms, cudaStream_t s) {
   p.out_type = a.out_type;
   p.kblocks = (int)((a.K + bk - 1) / bk);
   p.blocks_n = (int)scale_blocks(a.N);
-  // F32 accumulator; the type of A and B (f16 0, bf16 1, e4m3 0); M
+  // F32 accumulator; the type of A and B (f16 0, bf16 1, e4m3 0); M = 128
   const uint32_t fmt = a.type == ELEM_BF16 ? 1u : 0u;
-  p.idesc = (1u << 4) | (fmt << 7) | (fmt << 10) | ((uint32_t)((pair ? 256 : 128) >> 4) << 24);
+  p.idesc = (1u << 4) | (fmt << 7) | (fmt << 10) | ((uint32_t)(128 >> 4) << 24);
   p.vec_out = (uintptr_t)a.out % 16 == 0 && a.ldo * elem_size(a.out_type) % 16 == 0;
   p.err = a.err;
 #ifdef OCCAMY_TC_TIMERS
   p.timers = tc_timer_words();
 #endif
   const int BN = each <= 32 ? 32 : (each <= 64 ? 64 : (each <= 128 ? 128 : 256));
-  const int tile_m = wide ? (pair ? 256 : 128) : BN, tile_n = (wide ? 256 : PT_ROWS) / (gated ? 2 : 1);
+  const int tile_m = wide ? 128 : BN, tile_n = (wide ? 256 : PT_ROWS) / (gated ? 2 : 1);
   p.tiles_n = (int)((a.N + tile_n - 1) / tile_n);
   const int64_t most_tiles = std::min<int64_t>((std::min(a.groups, a.rows) + a.rows / tile_m) * p.tiles_n, 1 << 28);
-  if (wide) return launch_product_wide(p, gated, pair, most_tiles, num_sms, s);
+  if (wide) return launch_product_wide(p, gated, most_tiles, num_sms, s);
   switch (BN) {
     case 32: return launch_width<32>(p, scaled, gated, most_tiles, num_sms, s);
     case 64: return launch_width<64>(p, scaled, gated, most_tiles, num_sms, s);

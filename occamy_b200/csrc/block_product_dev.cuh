@@ -12,8 +12,16 @@ namespace occ {
 constexpr int PT_BOX = 32;             // rows of one copy
 constexpr int PT_RASTER = 16;          // row tiles that go through all weights together
 
+// Warps of either form: 0 loads, 1 MMAs, 2 and 3 scales, four that copy rows chosen by an index, eight of the epilogue, two
+// for each TMEM quadrant.
+constexpr int PT_GATHER_WARP = 4, PT_GATHERERS = 4, PT_EPI_WARP = 8, PT_EPI_WARPS = 8;
+constexpr int PT_THREADS = 32 * (PT_EPI_WARP + PT_EPI_WARPS);
+
 struct alignas(64) PtParams {
-  CUtensorMap ta, tb;
+  CUtensorMap ta, tb;                  // (ta: without an index)
+  const uint8_t *a;                    // with an index: A, units of 16 bytes from row to row, bytes in a row
+  uint32_t a_ld16;
+  int k_bytes;
   const int32_t *index, *offsets;
   const float *scale_a, *scale_b, *bias;
   void *out;
@@ -30,21 +38,16 @@ struct alignas(64) PtParams {
 #endif
 };
 
-// kind::f16, or kind::f8f6f4 for e4m3; by one CTA or a pair.
-template <bool E4M3, bool PAIR>
+// A tile of the result.
+struct PtTile {
+  int g, m0, rows, n0;   // group, first row, rows in the tile, first weight (of a gated pair)
+};
+
+// kind::f16, or kind::f8f6f4 for e4m3.
+template <bool E4M3>
 __device__ __forceinline__ void pt_mma(uint32_t d_tmem, uint32_t a_lo, uint32_t a_hi, uint32_t b_lo, uint32_t b_hi,
                                        uint32_t idesc, uint32_t accumulate) {
-  if constexpr (E4M3 && PAIR)
-    asm volatile(
-        "{\n.reg .pred p, q;\n.reg .b64 da, db;\n"
-        "elect.sync _|q, 0xffffffff;\n"
-        "setp.ne.b32 p, %6, 0;\n"
-        "mov.b64 da, {%1, %2};\n"
-        "mov.b64 db, {%3, %4};\n"
-        "@q tcgen05.mma.cta_group::2.kind::f8f6f4 [%0], da, db, %5, p;\n}" ::"r"(d_tmem),
-        "r"(a_lo), "r"(a_hi), "r"(b_lo), "r"(b_hi), "r"(idesc), "r"(accumulate)
-        : "memory");
-  else if constexpr (E4M3)
+  if constexpr (E4M3)
     asm volatile(
         "{\n.reg .pred p, q;\n.reg .b64 da, db;\n"
         "elect.sync _|q, 0xffffffff;\n"
@@ -54,73 +57,80 @@ __device__ __forceinline__ void pt_mma(uint32_t d_tmem, uint32_t a_lo, uint32_t 
         "@q tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], da, db, %5, p;\n}" ::"r"(d_tmem),
         "r"(a_lo), "r"(a_hi), "r"(b_lo), "r"(b_hi), "r"(idesc), "r"(accumulate)
         : "memory");
-  else if constexpr (PAIR)
-    mma_pair_warp(d_tmem, a_lo, a_hi, b_lo, b_hi, idesc, accumulate);
   else
     mma_warp(d_tmem, a_lo, a_hi, b_lo, b_hi, idesc, accumulate);
 }
-// Copies of two- and five-dimensional boxes; PAIR: counted on a barrier that may be the other CTA's (a shared::cluster
-// address; the data lands in the issuing CTA's own memory).
-template <bool PAIR>
 __device__ __forceinline__ void load_2d_warp(uint32_t dst, const CUtensorMap *m, uint32_t bar, int c0, int c1) {
-  if constexpr (PAIR)
-    asm volatile(
-        "{\n.reg .pred q;\nelect.sync _|q, 0xffffffff;\n"
-        "@q cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes "
-        "[%0], [%1, {%3, %4}], [%2];\n}" ::"r"(dst),
-        "l"(m), "r"(bar), "r"(c0), "r"(c1)
-        : "memory");
-  else
-    asm volatile(
-        "{\n.reg .pred q;\nelect.sync _|q, 0xffffffff;\n"
-        "@q cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];\n}" ::"r"(dst),
-        "l"(m), "r"(bar), "r"(c0), "r"(c1)
-        : "memory");
+  asm volatile(
+      "{\n.reg .pred q;\nelect.sync _|q, 0xffffffff;\n"
+      "@q cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];\n}" ::"r"(dst),
+      "l"(m), "r"(bar), "r"(c0), "r"(c1)
+      : "memory");
 }
-template <bool PAIR>
 __device__ __forceinline__ void load_5d_warp(uint32_t dst, const CUtensorMap *m, uint32_t bar, int c0, int c3, int c4) {
-  if constexpr (PAIR)
-    asm volatile(
-        "{\n.reg .pred q;\nelect.sync _|q, 0xffffffff;\n"
-        "@q cp.async.bulk.tensor.5d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes "
-        "[%0], [%1, {%3, %6, %6, %4, %5}], [%2];\n}" ::"r"(dst),
-        "l"(m), "r"(bar), "r"(c0), "r"(c3), "r"(c4), "r"(0)
-        : "memory");
-  else
-    asm volatile(
-        "{\n.reg .pred q;\nelect.sync _|q, 0xffffffff;\n"
-        "@q cp.async.bulk.tensor.5d.shared::cluster.global.mbarrier::complete_tx::bytes "
-        "[%0], [%1, {%3, %6, %6, %4, %5}], [%2];\n}" ::"r"(dst),
-        "l"(m), "r"(bar), "r"(c0), "r"(c3), "r"(c4), "r"(0)
-        : "memory");
+  asm volatile(
+      "{\n.reg .pred q;\nelect.sync _|q, 0xffffffff;\n"
+      "@q cp.async.bulk.tensor.5d.shared::cluster.global.mbarrier::complete_tx::bytes "
+      "[%0], [%1, {%3, %6, %6, %4, %5}], [%2];\n}" ::"r"(dst),
+      "l"(m), "r"(bar), "r"(c0), "r"(c3), "r"(c4), "r"(0)
+      : "memory");
 }
-// Four rows, by the executing lane.
-template <bool PAIR>
-__device__ __forceinline__ void gather_4_rows(uint32_t dst, const CUtensorMap *m, uint32_t bar, int c0, int4 r) {
-  if constexpr (PAIR)
-    asm volatile(
-        "cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.tile::gather4.mbarrier::complete_tx::bytes "
-        "[%0], [%1, {%3, %4, %5, %6, %7}], [%2];" ::"r"(dst),
-        "l"(m), "r"(bar), "r"(c0), "r"(r.x), "r"(r.y), "r"(r.z), "r"(r.w)
-        : "memory");
-  else
-    asm volatile(
-        "cp.async.bulk.tensor.2d.shared::cta.global.tile::gather4.mbarrier::complete_tx::bytes "
-        "[%0], [%1, {%3, %4, %5, %6, %7}], [%2];" ::"r"(dst),
-        "l"(m), "r"(bar), "r"(c0), "r"(r.x), "r"(r.y), "r"(r.z), "r"(r.w)
-        : "memory");
-}
-// Rows 4 i .. 4 i + 3 of a tile that begins at row m0 and has `rows`: where they are in A.  One that there is not, or none,
-// reads as zeros.
-__device__ __forceinline__ int4 four_rows(const PtParams &p, int m0, int rows, int i) {
-  int r[4];
+
+// ---- rows chosen by an index
+// Four warps copy them, 16 bytes a lane, in the swizzled order that the tensor core reads.  (TMA's own gather of four rows
+// takes 75 cycles an instruction, 2400 for the 128 rows of a k-step; a cp.async of a warp takes that warp 30 cycles, a k-step
+// by one warp 960 and with the epilogue beside it 3300.)  The copies arrive at the k-step's barrier by themselves, one arrival for
+// each lane, and the warp that issues the MMAs makes them visible to the tensor core.
+// The role of these warps, warp `warp` of WARPS.  A lane holds where its rows (4 j WARPS + 4 warp + lane / 8) begin,
+// in units of 16 bytes, for a whole tile.  Returns an error code.
+template <int ROWS, int WARPS, typename Decode, typename Full, typename Empty>
+__device__ __forceinline__ int pt_gather_role(const PtParams &p, int tile0, int total, int tstep, int k0, int k1, uint32_t sR,
+                                              int stages, int warp, int lane, volatile int *abort_flag, Decode &&decode,
+                                              Full &&full_bar, Empty &&empty_bar) {
+  constexpr int MINE = ROWS / (4 * WARPS);
+  static_assert(MINE <= 32, "a bit for each row");
+  int stage = 0, err = 0;
+  uint32_t phase = 0;
+  const int row0 = warp * 4 + (lane >> 3), chunk = lane & 7;
+  for (int tile = tile0; tile < total && !err; tile += tstep) {
+    const PtTile tl = decode(tile);
+    uint32_t begin[MINE], there = 0;
 #pragma unroll
-  for (int j = 0; j < 4; ++j) {
-    const int m = i * 4 + j;
-    r[j] = m < rows ? p.index[m0 + m] : -1;
-    if (r[j] < 0 || r[j] >= p.a_rows) r[j] = p.a_rows;
+    for (int j = 0; j < MINE; ++j) {
+      const int i = row0 + j * 4 * WARPS;
+      const int r = i < tl.rows ? p.index[tl.m0 + i] : -1;
+      const bool in = r >= 0 && r < p.a_rows;        // one that there is not reads as zeros
+      begin[j] = in ? (uint32_t)r * p.a_ld16 : 0u;
+      there |= (uint32_t)in << j;
+    }
+    const int mine = (tl.rows - row0 + 4 * WARPS - 1) / (4 * WARPS);   // (none: not positive)
+    for (int kb = k0; kb < k1; ++kb) {
+      if (!mbar_wait_warp(empty_bar(stage), phase ^ 1u, abort_flag)) {
+        err = 7;
+        break;
+      }
+      const int at = kb * 128 + chunk * 16;
+      const uint32_t have = (uint32_t)max(0, min(16, p.k_bytes - at));   // the rows end here: zeros behind them
+      const uint8_t *base = p.a + (have ? at : 0);
+      const uint32_t dst = sR + stage * (ROWS * 128u) + row0 * 128u;
+#pragma unroll
+      for (int j = 0; j < MINE; ++j)
+        if (j < mine) {
+          const uint32_t size = there >> j & 1u ? have : 0u;
+          asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(
+                           dst + (uint32_t)(j * WARPS * 512) + (uint32_t)((chunk ^ ((row0 + j * 4 * WARPS) & 7)) << 4)),
+                       "l"(base + ((uint64_t)begin[j] << 4)), "r"(size)
+                       : "memory");
+        }
+      asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(full_bar(stage)) : "memory");
+      if (++stage == stages) {
+        stage = 0;
+        phase ^= 1u;
+      }
+    }
   }
-  return make_int4(r[0], r[1], r[2], r[3]);
+  asm volatile("cp.async.wait_all;" ::: "memory");   // nothing may be under way when the CTA ends
+  return err;
 }
 __device__ __forceinline__ uint64_t f2_fma(uint64_t a, uint64_t b, uint64_t c) {
   uint64_t r;
@@ -147,9 +157,9 @@ __device__ __forceinline__ uint32_t pack16(float a, float b, int type) {
   return type == ELEM_F16 ? f2_to_bf16x2<true>(f2_pack(a, b)) : f2_to_bf16x2<false>(f2_pack(a, b));
 }
 // W results of one row, the first `have` of them; `out` is their address.
-template <int W>
+template <int W, bool WHOLE = false>
 __device__ __forceinline__ void store_row(const PtParams &p, uint8_t *out, const float *r, int have) {
-  if (p.vec_out && have >= W) {
+  if (WHOLE || (p.vec_out && have >= W)) {
     if (p.out_type == ELEM_F32) {
 #pragma unroll
       for (int j = 0; j < W; j += 4) *reinterpret_cast<float4 *>(out + j * 4) = make_float4(r[j], r[j + 1], r[j + 2], r[j + 3]);
@@ -169,10 +179,7 @@ __device__ __forceinline__ void store_row(const PtParams &p, uint8_t *out, const
   }
 }
 
-// Which rows a tile has, and whose.  Shared memory: first and last + 1 row of each group, row tiles before it.
-struct PtTile {
-  int g, m0, rows, n0;   // group, first row, rows in the tile, first weight (of a gated pair)
-};
+// Shared memory: first and last + 1 row of each group, row tiles before it.
 struct PtGroups {
   int32_t *first, *last, *before;
 };
@@ -226,7 +233,7 @@ __device__ __forceinline__ int pt_total(const PtParams &p, const PtGroups &t) {
   return (int)min((int64_t)t.before[p.groups] * p.tiles_n, (int64_t)0x7fffffff);
 }
 
-// block_product_wide.cu.  Rows of its tiles' M side; launch.
-cudaError_t launch_product_wide(PtParams &p, bool gated, bool pair, int64_t most_tiles, int num_sms, cudaStream_t s);
+// block_product_wide.cu
+cudaError_t launch_product_wide(PtParams &p, bool gated, int64_t most_tiles, int num_sms, cudaStream_t s);
 
 }  // namespace occ

@@ -148,7 +148,7 @@ bool linear_act(int64_t mode) {
 // The products' common part.  `rows`: of the result.
 int product(Call &call, ProductArgs &p, cudaStream_t stream) {
   const char *who = call.who();
-  if (!extent(p.a_rows) || !extent(p.rows) || !extent(p.N) || !extent(p.groups) || p.K < 1 || p.K > INT_MAX)
+  if (!extent(p.a_rows) || !extent(p.rows) || !extent(p.N) || !extent(p.groups) || p.K < 1 || p.K > INT_MAX / 2)
     return refuse(BAD_ARGUMENT, who, "extent out of range");
   const int both = p.act == ACT_GATED_SILU ? 2 : 1, es = elem_size(p.type);
   const int64_t mats = p.groups * both;
@@ -158,6 +158,8 @@ int product(Call &call, ProductArgs &p, cudaStream_t stream) {
     return refuse(BAD_ARGUMENT, who, "distance between rows out of range");
   if (p.lda * es % 16 || p.ldb * es % 16)
     return refuse(BAD_ARGUMENT, who, "rows of the operands have to start at multiples of 16 bytes");
+  if (p.index && p.a_rows * (p.lda * es / 16) > (int64_t)UINT32_MAX)
+    return refuse(BAD_ARGUMENT, who, "A of more than 64 GiB cannot be indexed");
   if (both == 2 && p.N % 8) return refuse(BAD_ARGUMENT, who, "a gated product needs N %% 8 == 0");
   const bool scaled = p.type == ELEM_E4M3;
   if (p.rows == 0 || p.N == 0) return 0;

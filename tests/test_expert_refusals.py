@@ -45,7 +45,7 @@ def test_matmul_refuses(lib, other):
 
 
 @pytest.mark.parametrize("other", [
-    dict(type=0), dict(type=4), dict(a_rows=9), dict(index=P, a_rows=-1), dict(index=P, a_rows=0), dict(rows=-1), dict(groups=-1), dict(groups=1025),
+    dict(type=0), dict(type=4), dict(a_rows=9), dict(index=P, a_rows=-1), dict(index=P, a_rows=0), dict(index=P, a_rows=1 << 30, lda=256), dict(rows=-1), dict(groups=-1), dict(groups=1025),
     dict(k=0), dict(act=4), dict(act=8), dict(act=7, n=20, ldo=20), dict(lda=260), dict(ldb=260), dict(out_type=3),
     dict(offsets=None), dict(a=None), dict(b=None), dict(out=None), dict(type=3), dict(type=3, scale_a=P),
     dict(groups=1024, n=1 << 22, ldo=1 << 22)])
