@@ -187,20 +187,110 @@ cudaError_t launch_choose(const RouteArgs &a, unsigned blocks, int64_t per_block
 }
 
 // ---------------------------------------------------------------- weighted sum
-__global__ void combine_kernel(CombineArgs a) {
+template <typename T>
+__device__ __forceinline__ float as_float(T v) {
+  if constexpr (sizeof(T) == 4) return v;
+  else return (float)v;
+}
+template <typename T>
+struct Row8 {   // eight elements of a row, in 16-byte pieces
+  uint4 w[sizeof(T) / 2];
+  __device__ __forceinline__ void load(const T *p) {
+#pragma unroll
+    for (int i = 0; i < (int)sizeof(T) / 2; ++i) w[i] = __ldcs(reinterpret_cast<const uint4 *>(p) + i);
+  }
+  __device__ __forceinline__ void add(float f, float *sum) const {
+    const T *e = reinterpret_cast<const T *>(w);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) sum[j] = fmaf(f, as_float(e[j]), sum[j]);
+  }
+};
+template <typename T>
+__device__ __forceinline__ void put8(T *p, const float *v) {
+  if constexpr (sizeof(T) == 4) {
+    reinterpret_cast<float4 *>(p)[0] = make_float4(v[0], v[1], v[2], v[3]);
+    reinterpret_cast<float4 *>(p)[1] = make_float4(v[4], v[5], v[6], v[7]);
+  } else {
+    T t[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) t[j] = (T)v[j];
+    *reinterpret_cast<uint4 *>(p) = *reinterpret_cast<const uint4 *>(t);
+  }
+}
+
+// Eight results a thread, the rows of four choices on their way together; `per_row` threads for each token.  Needs rows that begin
+// at multiples of 16 bytes; the last threads' elements beyond N one by one.
+template <typename T, typename O>
+__global__ void __launch_bounds__(256) combine_kernel(CombineArgs a, int per_row) {
   chain_begin();
+  const T *y = (const T *)a.y;
+  O *out = (O *)a.out;
+  const int64_t total = a.tokens * per_row;
+  for (int64_t i = blockIdx.x * (int64_t)256 + threadIdx.x; i < total; i += (int64_t)gridDim.x * 256) {
+    const int64_t t = total <= 0x7fffffff ? (int64_t)((uint32_t)i / (uint32_t)per_row) : i / per_row;
+    const int64_t n = (i - t * per_row) * 8;
+    const int32_t *position = a.position + t * a.k;
+    const float *weights = a.weights + t * a.k;
+    float sum[8] = {};
+    if (n + 8 <= a.N) {
+      for (int j0 = 0; j0 < a.k; j0 += 4) {
+        Row8<T> r[4];
+        bool there[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const int32_t at = j0 + j < a.k ? position[j0 + j] : -1;
+          there[j] = at >= 0 && at < a.y_rows;
+          if (there[j]) r[j].load(y + at * a.ldy + n);
+        }
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          if (there[j]) r[j].add(weights[j0 + j], sum);
+      }
+      put8(out + t * a.ldo + n, sum);
+    } else {
+      for (int e = 0; n + e < a.N; ++e) {
+        float v = 0.0f;
+        for (int j = 0; j < a.k; ++j) {
+          const int32_t at = position[j];
+          if (at >= 0 && at < a.y_rows) v = fmaf(weights[j], as_float(y[at * a.ldy + n + e]), v);
+        }
+        out[t * a.ldo + n + e] = (O)v;
+      }
+    }
+  }
+}
+// Rows that begin anywhere: one result a thread.
+template <typename T, typename O>
+__global__ void __launch_bounds__(256) combine_plain_kernel(CombineArgs a) {
+  chain_begin();
+  const T *y = (const T *)a.y;
   const int64_t total = a.tokens * a.N;
-  for (int64_t i = blockIdx.x * (int64_t)blockDim.x + threadIdx.x; i < total; i += (int64_t)gridDim.x * blockDim.x) {
+  for (int64_t i = blockIdx.x * (int64_t)256 + threadIdx.x; i < total; i += (int64_t)gridDim.x * 256) {
     const int64_t t = i / a.N, n = i % a.N;
     float sum = 0.0f;
-    for (int64_t j = 0; j < a.k; ++j) {
+    for (int j = 0; j < a.k; ++j) {
       const int32_t at = a.position[t * a.k + j];
-      if (at >= 0 && at < a.y_rows) sum = fmaf(a.weights[t * a.k + j], load_logit(a.y, at * a.ldy + n, a.type), sum);
+      if (at >= 0 && at < a.y_rows) sum = fmaf(a.weights[t * a.k + j], as_float(y[at * a.ldy + n]), sum);
     }
-    if (a.out_type == ELEM_F32) ((float *)a.out)[t * a.ldo + n] = sum;
-    else if (a.out_type == ELEM_BF16) ((__nv_bfloat16 *)a.out)[t * a.ldo + n] = __float2bfloat16_rn(sum);
-    else ((__half *)a.out)[t * a.ldo + n] = __float2half_rn(sum);
+    ((O *)a.out)[t * a.ldo + n] = (O)sum;
   }
+}
+
+template <typename T, typename O>
+cudaError_t launch_sum(const CombineArgs &a, int num_sms, cudaStream_t s) {
+  const bool vec = (uintptr_t)a.y % 16 == 0 && a.ldy * sizeof(T) % 16 == 0 && (uintptr_t)a.out % 16 == 0 &&
+                   a.ldo * sizeof(O) % 16 == 0;
+  const int per_row = vec ? (int)((a.N + 7) / 8) : (int)a.N;
+  const int64_t want = (a.tokens * per_row + 255) / 256, most = (int64_t)num_sms * 64;
+  const dim3 grid((unsigned)(want < most ? want : most));
+  return vec ? launch_after(combine_kernel<T, O>, grid, dim3(256), 0, s, 1, a, per_row)
+             : launch_after(combine_plain_kernel<T, O>, grid, dim3(256), 0, s, 1, a);
+}
+template <typename T>
+cudaError_t launch_sum_of(const CombineArgs &a, int num_sms, cudaStream_t s) {
+  if (a.out_type == ELEM_F32) return launch_sum<T, float>(a, num_sms, s);
+  if (a.out_type == ELEM_BF16) return launch_sum<T, __nv_bfloat16>(a, num_sms, s);
+  return launch_sum<T, __half>(a, num_sms, s);
 }
 
 }  // namespace
@@ -225,8 +315,9 @@ cudaError_t launch_route(const RouteArgs &a, cudaStream_t s) {
 }
 
 cudaError_t launch_combine(const CombineArgs &a, int num_sms, cudaStream_t s) {
-  const int64_t want = (a.tokens * a.N + 255) / 256, most = (int64_t)num_sms * 32;
-  return launch_after(combine_kernel, dim3((unsigned)(want < most ? want : most)), dim3(256), 0, s, 1, a);
+  if (a.type == ELEM_F32) return launch_sum_of<float>(a, num_sms, s);
+  if (a.type == ELEM_BF16) return launch_sum_of<__nv_bfloat16>(a, num_sms, s);
+  return launch_sum_of<__half>(a, num_sms, s);
 }
 
 }  // namespace occ
