@@ -3,6 +3,8 @@
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
+#include <type_traits>
+
 #include "expert_ops.h"
 #include "kernels.h"
 
@@ -12,18 +14,13 @@ namespace {
 constexpr int RT_THREADS = 1024, RT_WARPS = RT_THREADS / 32;
 constexpr int RT_TOKENS = 128;       // of a block, more when there would be over RT_BLOCKS of them
 constexpr int RT_BLOCKS = 256;
-constexpr int RT_MOST_EXPERTS = 1024;
+constexpr int PL_WARPS = 8;          // that count and place a block's rows
 
 inline int64_t tokens_of_block(int64_t tokens) {
   const int64_t even = (tokens + RT_BLOCKS - 1) / RT_BLOCKS;
   return even > RT_TOKENS ? even : RT_TOKENS;
 }
 
-__device__ __forceinline__ float load_logit(const void *p, int64_t i, int type) {
-  if (type == ELEM_F32) return ((const float *)p)[i];
-  if (type == ELEM_BF16) return __bfloat162float(((const __nv_bfloat16 *)p)[i]);
-  return __half2float(((const __half *)p)[i]);
-}
 // Unsigned keys in the order of the values; both zeros alike, every NaN above everything.
 __device__ __forceinline__ uint32_t key_of(float v) {
   if (v != v) return 0xffffffffu;
@@ -34,6 +31,25 @@ __device__ __forceinline__ float value_of(uint32_t k) {
   return __uint_as_float(k & 0x80000000u ? k & 0x7fffffffu : ~k);
 }
 constexpr uint32_t KEY_NONE = 0x007fffffu;   // of -inf: an expert that is not to be taken, and all below it
+// The same for 16-bit logits, whose key leaves room for the expert (the lower one the larger) in the same word: one comparison
+// of words does both.
+template <typename T>
+__device__ __forceinline__ uint32_t word_of(T v, int e) {
+  uint32_t b = *reinterpret_cast<const uint16_t *>(&v);
+  const float f = (float)v;
+  if (b == 0x8000u) b = 0;
+  b = f != f ? 0xffffu : (b & 0x8000u ? ~b & 0xffffu : b | 0x8000u);
+  return b << 16 | (0xffffu - (uint32_t)e);
+}
+template <typename T>
+__device__ __forceinline__ float value_of_word(uint32_t w) {
+  const uint32_t k = w >> 16;
+  const uint16_t b = (uint16_t)(k & 0x8000u ? k & 0x7fffu : ~k);
+  return (float)*reinterpret_cast<const T *>(&b);
+}
+// of -inf and the largest expert number: below every word of a value
+template <typename T>
+constexpr uint32_t WORD_NONE = std::is_same<T, __half>::value ? 0x03ffffffu : 0x007fffffu;
 
 __device__ __forceinline__ float warp_sum(float v) {
 #pragma unroll
@@ -41,43 +57,82 @@ __device__ __forceinline__ float warp_sum(float v) {
   return v;
 }
 
-// The k largest logits of token t, by one warp; lane j gets the j-th choice.  V = ceil(experts / 32).
-template <int V>
+// The k largest logits of token t, by one warp; lane j gets the j-th choice.  V = ceil(experts / 32), the numbers of a lane.
+//
+// 16-bit logits: a lane sorts its words, so that a choice looks at the first of each lane alone: one warp maximum, and the lane that had
+// it moves on (16384 tokens, 128 experts, k = 8: 20 us with all words looked at for every choice, this way PLACEHOLDER).  fp32: the
+// lanes look through theirs, and the lowest expert among equals comes from a second warp minimum.
+template <typename T, int V>
 __device__ __forceinline__ void choose(const RouteArgs &a, int64_t t, int lane) {
+  constexpr bool WORDS = sizeof(T) == 2;
+  const T *logits = (const T *)a.logits + t * a.ldl;
   uint32_t key[V];
 #pragma unroll
   for (int v = 0; v < V; ++v) {
     const int e = v * 32 + lane;
-    key[v] = e < a.experts ? key_of(load_logit(a.logits, t * a.ldl + e, a.type)) : 0u;
+    if constexpr (WORDS) key[v] = e < a.experts ? word_of(logits[e], e) : 0u;
+    else key[v] = e < a.experts ? key_of(logits[e]) : 0u;
   }
+  auto value = [](uint32_t k) {
+    if constexpr (WORDS) return value_of_word<T>(k);
+    else return value_of(k);
+  };
+  constexpr uint32_t none = WORDS ? WORD_NONE<T> : KEY_NONE;
   uint32_t mine = 0;
   int expert = -1;
   float top = 0.0f, total = 0.0f;
-  for (int j = 0; j < a.k; ++j) {
-    uint32_t best = 0;
-    int at = 0;
+  auto sum_all = [&] {   // behind the first choice
+    float sum = 0.0f;
 #pragma unroll
     for (int v = 0; v < V; ++v)
-      if (key[v] > best) best = key[v], at = v * 32 + lane;
-    const uint32_t high = __reduce_max_sync(0xffffffffu, best);
-    if (high <= KEY_NONE) break;
-    const int e = (int)__reduce_min_sync(0xffffffffu, best == high ? (uint32_t)at : 0xffffffffu);
-    if (j == 0) {
-      top = value_of(high);
-      if (!a.normalise) {
-        float sum = 0.0f;
+      if (key[v] > none) sum += expf(value(key[v]) - top);
+    total = warp_sum(sum);
+  };
+  if constexpr (WORDS && V <= 8) {
+    // odd-even transposition: V rounds
 #pragma unroll
-        for (int v = 0; v < V; ++v)
-          if (key[v] > KEY_NONE) sum += expf(value_of(key[v]) - top);
-        total = warp_sum(sum);
+    for (int r = 0; r < V; ++r)
+#pragma unroll
+      for (int v = r & 1; v + 1 < V; v += 2) {
+        const uint32_t hi = max(key[v], key[v + 1]), lo = min(key[v], key[v + 1]);
+        key[v] = hi;
+        key[v + 1] = lo;
+      }
+    for (int j = 0; j < a.k; ++j) {
+      const uint32_t high = __reduce_max_sync(0xffffffffu, key[0]);
+      if (high <= none) break;
+      if (j == 0) {
+        top = value(high);
+        if (!a.normalise) sum_all();
+      }
+      if (lane == j) mine = high, expert = (int)(0xffffu - (high & 0xffffu));
+      if (key[0] == high) {
+#pragma unroll
+        for (int v = 0; v + 1 < V; ++v) key[v] = key[v + 1];
+        key[V - 1] = 0;
       }
     }
-    if (lane == j) mine = high, expert = e;
+  } else {
+    for (int j = 0; j < a.k; ++j) {
+      uint32_t best = 0;
+      int at = 0;
 #pragma unroll
-    for (int v = 0; v < V; ++v)
-      if (e == v * 32 + lane) key[v] = 0;
+      for (int v = 0; v < V; ++v)
+        if (key[v] > best) best = key[v], at = v * 32 + lane;
+      const uint32_t high = __reduce_max_sync(0xffffffffu, best);
+      if (high <= none) break;
+      const int e = (int)__reduce_min_sync(0xffffffffu, best == high ? (uint32_t)at : 0xffffffffu);
+      if (j == 0) {
+        top = value(high);
+        if (!a.normalise) sum_all();
+      }
+      if (lane == j) mine = high, expert = e;
+#pragma unroll
+      for (int v = 0; v < V; ++v)
+        if (e == v * 32 + lane) key[v] = 0;
+    }
   }
-  float w = expert >= 0 ? expf(value_of(mine) - top) : 0.0f;
+  float w = expert >= 0 ? expf(value(mine) - top) : 0.0f;
   if (a.normalise) total = warp_sum(w);
   if (expert >= 0) w /= total;
   if (lane < a.k) {
@@ -86,60 +141,120 @@ __device__ __forceinline__ void choose(const RouteArgs &a, int64_t t, int lane) 
   }
 }
 
-template <int V>
+template <typename T, int V>
 __device__ __forceinline__ void choose_block(const RouteArgs &a, int64_t t0, int64_t t1) {
-  for (int64_t t = t0 + (threadIdx.x >> 5); t < t1; t += RT_WARPS) choose<V>(a, t, threadIdx.x & 31);
+  for (int64_t t = t0 + (threadIdx.x >> 5); t < t1; t += RT_WARPS) choose<T, V>(a, t, threadIdx.x & 31);
 }
 
-// Rows of this block's (token, choice) slots: they go behind base[expert] in the order of the slots.  Each warp counts its
-// share of the slots first; after that every one knows where its own begin.  cnt: [warps][experts] in shared memory.
-__device__ __forceinline__ void place_block(const RouteArgs &a, int64_t s0, int64_t s1, const int32_t *base, int32_t *cnt,
-                                            int warps) {
-  const int E = (int)a.experts, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int64_t share = ((s1 - s0 + warps - 1) / warps + 31) / 32 * 32;
-  const int64_t w0 = s0 + warp * share, w1 = w0 + share < s1 ? w0 + share : s1;
-  for (int i = threadIdx.x; i < warps * E; i += RT_THREADS) cnt[i] = 0;
+// Exclusive prefix sums of one number for each thread; `sums`: 32 words of shared memory.  The last thread's result and number
+// make the total.
+__device__ __forceinline__ int scan_block(int n, int32_t *sums) {
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  int upto = n;
+#pragma unroll
+  for (int d = 1; d < 32; d *= 2) {
+    const int o = __shfl_up_sync(0xffffffffu, upto, d);
+    if (lane >= d) upto += o;
+  }
+  if (lane == 31) sums[warp] = upto;
   __syncthreads();
-  if (warp < warps)
-    for (int64_t s = w0 + lane; s < w1; s += 32) {
+  if (warp == 0) {
+    int t = sums[lane];
+#pragma unroll
+    for (int d = 1; d < 32; d *= 2) {
+      const int o = __shfl_up_sync(0xffffffffu, t, d);
+      if (lane >= d) t += o;
+    }
+    sums[lane] = t;
+  }
+  __syncthreads();
+  return upto - n + (warp ? sums[warp - 1] : 0);
+}
+
+// The slots (token, choice) [s0, s1) of a block, shared out to `warps` of its warps in whole groups of 32.
+struct Slots {
+  int64_t from, to;
+};
+__device__ __forceinline__ Slots slots_of(int64_t s0, int64_t s1, int warp, int warps) {
+  const int64_t share = ((s1 - s0 + warps - 1) / warps + 31) / 32 * 32;
+  const int64_t from = s0 + warp * share, to = from + share;
+  return {from, to < s1 ? to : s1};
+}
+// cnt [warps][experts], in shared memory: how many rows each warp's slots bring to each expert.
+__device__ __forceinline__ void count_slots(const RouteArgs &a, int64_t s0, int64_t s1, int32_t *cnt) {
+  const int E = (int)a.experts, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  for (int i = threadIdx.x; i < PL_WARPS * E; i += RT_THREADS) cnt[i] = 0;
+  __syncthreads();
+  if (warp < PL_WARPS) {
+    const Slots mine = slots_of(s0, s1, warp, PL_WARPS);
+    for (int64_t s = mine.from + lane; s < mine.to; s += 32) {
       const int e = a.chosen[s];
       if (e >= 0) atomicAdd(&cnt[warp * E + e], 1);
     }
+  }
   __syncthreads();
-  for (int e = threadIdx.x; e < E; e += RT_THREADS) {
-    int at = base[e];
-    for (int w = 0; w < warps; ++w) {
-      const int n = cnt[w * E + e];
-      cnt[w * E + e] = at;
-      at += n;
+}
+// Their rows: those of expert e go behind base (this thread's, e == threadIdx.x) in the order of the slots.
+__device__ __forceinline__ void place_slots(const RouteArgs &a, int64_t s0, int64_t s1, int base, int32_t *cnt) {
+  const int E = (int)a.experts, warp = threadIdx.x >> 5, lane = threadIdx.x & 31, e0 = threadIdx.x;
+  if (e0 < E) {
+    int n[PL_WARPS];
+#pragma unroll
+    for (int w = 0; w < PL_WARPS; ++w) n[w] = cnt[w * E + e0];
+#pragma unroll
+    for (int w = 0; w < PL_WARPS; ++w) {
+      cnt[w * E + e0] = base;
+      base += n[w];
     }
   }
   __syncthreads();
-  if (warp < warps)
-    for (int64_t s = w0; s < w1; s += 32) {
-      const bool in = s + lane < w1;
-      const int e = in ? a.chosen[s + lane] : -1;
-      const unsigned same = __match_any_sync(0xffffffffu, e);
-      const int before = __popc(same & ((1u << lane) - 1u));
-      int at = -1;
-      if (e >= 0) at = cnt[warp * E + e] + before;
-      __syncwarp();
-      if (e >= 0 && before == 0) cnt[warp * E + e] += __popc(same);
-      __syncwarp();
-      if (in) a.position[s + lane] = at;
-      if (at >= 0) a.order[at] = (int32_t)((s + lane) / a.k);
-    }
+  if (warp >= PL_WARPS) return;
+  const Slots mine = slots_of(s0, s1, warp, PL_WARPS);
+  for (int64_t s = mine.from; s < mine.to; s += 32) {
+    const bool in = s + lane < mine.to;
+    const int e = in ? a.chosen[s + lane] : -1;
+    const unsigned same = __match_any_sync(0xffffffffu, e);
+    const int before = __popc(same & ((1u << lane) - 1u));
+    int at = -1;
+    if (e >= 0) at = cnt[warp * E + e] + before;
+    __syncwarp();
+    if (e >= 0 && before == 0) cnt[warp * E + e] += __popc(same);
+    __syncwarp();
+    if (in) a.position[s + lane] = at;
+    if (at >= 0) a.order[at] = (int32_t)((s + lane) / a.k);
+  }
+}
+// All of it, for tokens that one block takes.
+template <typename T, int V>
+__global__ void __launch_bounds__(RT_THREADS) route_one_kernel(RouteArgs a) {
+  extern __shared__ int32_t cnt[];
+  __shared__ int32_t sums[32];
+  chain_begin();
+  const int E = (int)a.experts, e = threadIdx.x;
+  const int64_t slots = a.tokens * a.k;
+  choose_block<T, V>(a, 0, a.tokens);
+  __syncthreads();
+  count_slots(a, 0, slots, cnt);
+  int n = 0;
+  if (e < E) {
+#pragma unroll
+    for (int w = 0; w < PL_WARPS; ++w) n += cnt[w * E + e];
+  }
+  const int base = scan_block(n, sums);
+  if (e < E) a.offsets[e] = base;
+  const int used = sums[31];
+  if (e == 0) a.offsets[E] = used;
+  for (int64_t i = used + e; i < slots; i += RT_THREADS) a.order[i] = -1;
+  place_slots(a, 0, slots, base, cnt);
 }
 
-inline __host__ __device__ int place_warps(int64_t experts) { return experts <= 256 ? RT_WARPS : 8; }
-
-template <int V>
+template <typename T, int V>
 __global__ void __launch_bounds__(RT_THREADS) route_choose_kernel(RouteArgs a, int64_t per_block) {
   extern __shared__ int32_t cnt[];
   chain_begin();
   const int64_t t0 = blockIdx.x * per_block, t1 = t0 + per_block < a.tokens ? t0 + per_block : a.tokens;
   for (int e = threadIdx.x; e < a.experts; e += RT_THREADS) cnt[e] = 0;
-  choose_block<V>(a, t0, t1);
+  choose_block<T, V>(a, t0, t1);
   __syncthreads();
   for (int64_t s = t0 * a.k + threadIdx.x; s < t1 * a.k; s += RT_THREADS) {
     const int e = a.chosen[s];
@@ -151,39 +266,58 @@ __global__ void __launch_bounds__(RT_THREADS) route_choose_kernel(RouteArgs a, i
 
 __global__ void __launch_bounds__(RT_THREADS) route_place_kernel(RouteArgs a, int64_t per_block) {
   extern __shared__ int32_t sm[];
+  __shared__ int32_t sums[32];
   chain_begin();
-  const int E = (int)a.experts;
-  int32_t *base = sm, *total = sm + E, *cnt = sm + 2 * E;
+  const int E = (int)a.experts, e0 = threadIdx.x;
+  int32_t *front = sm, *total = sm + E, *cnt = sm + 2 * E;
   for (int e = threadIdx.x; e < 2 * E; e += RT_THREADS) sm[e] = 0;
   __syncthreads();
-  for (int64_t i = threadIdx.x; i < (int64_t)gridDim.x * E; i += RT_THREADS) {
-    const int e = (int)(i % E), n = a.counts[i];
-    if (!n) continue;
-    atomicAdd(&total[e], n);
-    if (i / E < blockIdx.x) atomicAdd(&base[e], n);
-  }
-  __syncthreads();
-  if (threadIdx.x == 0) {
-    int at = 0;
-    for (int e = 0; e < E; ++e) {
-      if (blockIdx.x == 0) a.offsets[e] = at;
-      base[e] += at;
-      at += total[e];
+  // rows of each expert in front of this block's, and of all: each thread adds up every RT_THREADS / E-th block
+  const int parts = RT_THREADS / E, part = e0 / E, e = e0 - part * E;
+  if (part < parts) {
+    int before = 0, all = 0;
+#pragma unroll 4
+    for (int b = part; b < (int)gridDim.x; b += parts) {
+      const int n = a.counts[b * E + e];
+      all += n;
+      before += b < (int)blockIdx.x ? n : 0;
     }
-    if (blockIdx.x == 0) a.offsets[E] = at;
-    total[0] = at;
+    atomicAdd(&front[e], before);
+    atomicAdd(&total[e], all);
   }
-  __syncthreads();
-  const int64_t used = total[0], all = a.tokens * a.k;
+  const int64_t t0 = blockIdx.x * per_block, t1 = t0 + per_block < a.tokens ? t0 + per_block : a.tokens;
+  count_slots(a, t0 * a.k, t1 * a.k, cnt);   // (its barriers come between the sums above and what follows)
+  const int first = scan_block(e0 < E ? total[e0] : 0, sums);
+  const int used = sums[31];
+  if (blockIdx.x == 0) {
+    if (e0 < E) a.offsets[e0] = first;
+    if (e0 == 0) a.offsets[E] = used;
+  }
+  const int64_t all = a.tokens * a.k;
   for (int64_t i = used + blockIdx.x * (int64_t)RT_THREADS + threadIdx.x; i < all; i += (int64_t)gridDim.x * RT_THREADS)
     a.order[i] = -1;
-  const int64_t t0 = blockIdx.x * per_block, t1 = t0 + per_block < a.tokens ? t0 + per_block : a.tokens;
-  place_block(a, t0 * a.k, t1 * a.k, base, cnt, place_warps(E));
+  place_slots(a, t0 * a.k, t1 * a.k, first + (e0 < E ? front[e0] : 0), cnt);
 }
 
-template <int V>
-cudaError_t launch_choose(const RouteArgs &a, unsigned blocks, int64_t per_block, cudaStream_t s) {
-  return launch_after(route_choose_kernel<V>, dim3(blocks), dim3(RT_THREADS), (size_t)a.experts * 4, s, 1, a, per_block);
+template <typename T, int V>
+cudaError_t launch_route_of(const RouteArgs &a, cudaStream_t s) {
+  const int64_t per = tokens_of_block(a.tokens);
+  const unsigned blocks = (unsigned)((a.tokens + per - 1) / per);
+  const size_t cnt = (size_t)a.experts * 4 * PL_WARPS;
+  if (blocks == 1) return launch_after(route_one_kernel<T, V>, dim3(1), dim3(RT_THREADS), cnt, s, 1, a);
+  const cudaError_t e =
+      launch_after(route_choose_kernel<T, V>, dim3(blocks), dim3(RT_THREADS), (size_t)a.experts * 4, s, 1, a, per);
+  if (e != cudaSuccess) return e;
+  return launch_after(route_place_kernel, dim3(blocks), dim3(RT_THREADS), cnt + (size_t)a.experts * 8, s, 1, a, per);
+}
+
+template <typename T>
+cudaError_t launch_route_typed(const RouteArgs &a, cudaStream_t s) {
+  if (a.experts <= 32) return launch_route_of<T, 1>(a, s);
+  if (a.experts <= 64) return launch_route_of<T, 2>(a, s);
+  if (a.experts <= 128) return launch_route_of<T, 4>(a, s);
+  if (a.experts <= 256) return launch_route_of<T, 8>(a, s);
+  return launch_route_of<T, 32>(a, s);
 }
 
 // ---------------------------------------------------------------- weighted sum
@@ -301,17 +435,9 @@ size_t route_workspace(int64_t tokens, int64_t experts, int64_t) {
 }
 
 cudaError_t launch_route(const RouteArgs &a, cudaStream_t s) {
-  const int64_t per = tokens_of_block(a.tokens);
-  const unsigned blocks = (unsigned)((a.tokens + per - 1) / per);
-  cudaError_t e;
-  if (a.experts <= 32) e = launch_choose<1>(a, blocks, per, s);
-  else if (a.experts <= 64) e = launch_choose<2>(a, blocks, per, s);
-  else if (a.experts <= 128) e = launch_choose<4>(a, blocks, per, s);
-  else if (a.experts <= 256) e = launch_choose<8>(a, blocks, per, s);
-  else e = launch_choose<32>(a, blocks, per, s);
-  if (e != cudaSuccess) return e;
-  const size_t smem = (size_t)a.experts * 4 * (2 + place_warps(a.experts));
-  return launch_after(route_place_kernel, dim3(blocks), dim3(RT_THREADS), smem, s, 1, a, per);
+  if (a.type == ELEM_F32) return launch_route_typed<float>(a, s);
+  if (a.type == ELEM_BF16) return launch_route_typed<__nv_bfloat16>(a, s);
+  return launch_route_typed<__half>(a, s);
 }
 
 cudaError_t launch_combine(const CombineArgs &a, int num_sms, cudaStream_t s) {
