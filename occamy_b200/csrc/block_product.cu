@@ -28,9 +28,9 @@ namespace {
 constexpr int PT_ROWS = 128;           // weights of a tile
 constexpr int PT_PER = 4;              // k-steps of 16-bit operands that the tensor core adds up by itself
 
-__device__ __forceinline__ float ld_cluster_f32(uint32_t addr) {
-  float v;
-  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(addr) : "memory");
+__device__ __forceinline__ float2 ld_cluster_f32x2(uint32_t addr) {
+  float2 v;
+  asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];" : "=f"(v.x), "=f"(v.y) : "r"(addr) : "memory");
   return v;
 }
 
@@ -435,14 +435,21 @@ __global__ void __launch_bounds__(PT_THREADS, BN <= 64 ? 2 : 1) block_product_ke
 #pragma unroll 1
         for (int g = 0; g < NG && c0 + g * 8 < tl.rows; ++g) {
           if ((ew * NG + g) % splits != rank) continue;
+          // (four CTAs' sums on their way together: one after another took 2 us)
           float t[8] = {};
-          for (int r = 0; r < splits; ++r) {
-            const uint32_t from = cluster_map(sW, (uint32_t)r) + (uint32_t)(g * 4 * EW * 32 + (int)threadIdx.x - 32 * PT_EPI_WARP) * 8u;
+          const uint32_t from = sW + (uint32_t)(g * 4 * EW * 32 + (int)threadIdx.x - 32 * PT_EPI_WARP) * 8u;
+          for (int r0 = 0; r0 < splits; r0 += 4) {
+            float2 x[4][4];
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-              t[2 * j] += ld_cluster_f32(from + j * (EW * 32 * 8));
-              t[2 * j + 1] += ld_cluster_f32(from + j * (EW * 32 * 8) + 4);
-            }
+            for (int r = 0; r < 4; ++r)
+#pragma unroll
+              for (int j = 0; j < 4; ++j)
+                x[r][j] = r0 + r < splits ? ld_cluster_f32x2(cluster_map(from, (uint32_t)(r0 + r)) + j * (EW * 32 * 8))
+                                          : make_float2(0.0f, 0.0f);
+#pragma unroll
+            for (int r = 0; r < 4; ++r)
+#pragma unroll
+              for (int j = 0; j < 4; ++j) t[2 * j] += x[r][j].x, t[2 * j + 1] += x[r][j].y;
           }
           finish(tl, g, [&](int, auto &&put) {
 #pragma unroll
@@ -494,7 +501,11 @@ cudaError_t launch_tiles(PtParams &p, int64_t most_tiles, int num_sms, cudaStrea
   const size_t misc = EW * 1024 + (SCALED ? p.bufs * (GATED ? 2 : 1) * BN * 4 : 0) + 8 * 3 * 4 + 16 +
                       (3 * (size_t)p.groups + 1) * 4;
   const size_t stage = (PT_ROWS + BN) * 128 + 16;
-  p.stages = (int)std::min<size_t>((LIMIT - misc) / stage, 16);
+  size_t limit = LIMIT;
+#ifdef OCCAMY_TUNING
+  if (getenv("OCCAMY_PT_SMEM")) limit = TC_SMEM_LIMIT;
+#endif
+  p.stages = (int)std::min<size_t>((limit - misc) / stage, 16);
   const size_t smem = p.stages * stage + misc;
   // the attribute is the device's: set for each once
   static std::once_flag once[64];
@@ -502,12 +513,24 @@ cudaError_t launch_tiles(PtParams &p, int64_t most_tiles, int num_sms, cudaStrea
   cudaError_t e = cudaGetDevice(&dev);
   if (e != cudaSuccess) return e;
   std::call_once(once[dev & 63], [] {
-    cudaFuncSetAttribute(block_product_kernel<BN, SCALED, GATED>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)LIMIT);
+    cudaFuncSetAttribute(block_product_kernel<BN, SCALED, GATED>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)TC_SMEM_LIMIT);
+    cudaFuncSetAttribute(block_product_kernel<BN, SCALED, GATED>, cudaFuncAttributePreferredSharedMemoryCarveout, cudaSharedmemCarveoutMaxShared);
   });
   const int64_t resident = (int64_t)num_sms * (BN <= 64 ? 2 : 1);
   p.splits = 1;
   if constexpr (BN <= 128)
     while (p.splits < 8 && most_tiles * p.splits * 2 <= resident && p.kblocks >= p.splits * 8) p.splits *= 2;
+#ifdef OCCAMY_TUNING
+  if (const char *e = getenv("OCCAMY_PT_SPLITS")) p.splits = atoi(e);
+  if (getenv("OCCAMY_PT_LOG")) {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)(most_tiles * p.splits)); cfg.blockDim = dim3(PT_THREADS); cfg.dynamicSmemBytes = smem;
+    cudaLaunchAttribute at; at.id = cudaLaunchAttributeClusterDimension; at.val.clusterDim.x = p.splits; at.val.clusterDim.y = at.val.clusterDim.z = 1;
+    cfg.attrs = &at; cfg.numAttrs = 1; int n = -1;
+    cudaOccupancyMaxActiveClusters(&n, block_product_kernel<BN, SCALED, GATED>, &cfg);
+    fprintf(stderr, "BN %d tiles %ld splits %d stages %d smem %zu: %d clusters fit\n", BN, (long)most_tiles, p.splits, p.stages, smem, n);
+  }
+#endif
   const int64_t grid = p.splits > 1 ? most_tiles * p.splits : std::min<int64_t>(most_tiles, resident);
   return launch_after(block_product_kernel<BN, SCALED, GATED>, dim3((unsigned)grid), dim3(PT_THREADS), smem, s,
                       p.splits, p);
@@ -579,7 +602,9 @@ cudaError_t launch_product(const ProductArgs &a, int num_sms, cudaStream_t s) {
   const int BN = each <= 32 ? 32 : (each <= 64 ? 64 : (each <= 128 ? 128 : 256));
   const int tile_m = wide ? 128 : BN, tile_n = (wide ? 256 : PT_ROWS) / (gated ? 2 : 1);
   p.tiles_n = (int)((a.N + tile_n - 1) / tile_n);
-  const int64_t most_tiles = std::min<int64_t>((std::min(a.groups, a.rows) + a.rows / tile_m) * p.tiles_n, 1 << 28);
+  // (rows of g groups fill at most so many tiles)
+  const int64_t most_tiles =
+      std::min<int64_t>((a.rows + std::min(a.groups, a.rows) * (tile_m - 1)) / tile_m * p.tiles_n, 1 << 28);
   if (wide) return launch_product_wide(p, gated, most_tiles, num_sms, s);
   switch (BN) {
     case 32: return launch_width<32>(p, scaled, gated, most_tiles, num_sms, s);

@@ -441,6 +441,7 @@ cudaError_t launch(PtParams &p, int64_t most_tiles, int num_sms, cudaStream_t s)
   if (e != cudaSuccess) return e;
   std::call_once(once[dev & 63], [] {
     cudaFuncSetAttribute(block_product_wide_kernel<GATED>, cudaFuncAttributeMaxDynamicSharedMemorySize, TC_SMEM_LIMIT);
+    cudaFuncSetAttribute(block_product_wide_kernel<GATED>, cudaFuncAttributePreferredSharedMemoryCarveout, cudaSharedmemCarveoutMaxShared);
   });
   return launch_after(block_product_wide_kernel<GATED>, dim3((unsigned)std::min<int64_t>(most_tiles, num_sms)), dim3(PT_THREADS),
                       p.stages * stage + misc, s, 1, p);
