@@ -16,6 +16,7 @@
 // With few tiles the CTAs of a cluster share a tile's K and add up their sums in rank order through each other's
 // shared memory: no workspace, and the same bits every time.
 #include <algorithm>
+#include <cmath>
 #include <cstring>
 #include <mutex>
 
@@ -39,7 +40,7 @@ __global__ void __launch_bounds__(PT_THREADS, BN <= 64 ? 2 : 1) block_product_ke
   constexpr int EW = PT_EPI_WARPS;
   constexpr int CW = BN / (EW / 4);      // columns of an epilogue warp
   constexpr int NG = CW / 8;             // groups of eight of them
-  constexpr int LD = CW < 32 ? CW : 32;  // columns of one TMEM load
+  constexpr int LD = CW == 32 ? 32 : 16;  // columns of one TMEM load (128 sums leave no registers for more)
   constexpr int SETS = GATED ? 2 : 1;    // scales of a column: first and second matrix
   constexpr int TILE_N = GATED ? PT_ROWS / 2 : PT_ROWS;
   extern __shared__ __align__(1024) uint8_t smem_raw[];
@@ -89,11 +90,7 @@ __global__ void __launch_bounds__(PT_THREADS, BN <= 64 ? 2 : 1) block_product_ke
                  : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
   }
-  pdl_launch_dependents();
-  pdl_wait();
-  pt_read_groups<PT_THREADS>(p, groups);
-  __syncthreads();
-  if (warp == 0) pt_count_tiles<BN>(p, groups, lane);
+  pt_find_groups<PT_THREADS, BN>(p, groups, lane);
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
@@ -493,6 +490,41 @@ bool encode(CUtensorMap *m, int type, const void *ptr, int rank, const cuuint64_
                    CUDA_SUCCESS;
 }
 
+// CTAs that share a tile's K: as many as there is room for, eight k-steps for each.
+int shares_of_k(int64_t tiles, int64_t resident, int kblocks) {
+  int s = 1;
+  while (s < 8 && tiles * s * 2 <= resident && kblocks >= s * 8) s *= 2;
+  return s;
+}
+
+// Rows of a tile: 32, 64, 128 (e4m3; with 16 bits two CTAs of 64 were as fast) with the rows on the N side, two CTAs of the first two
+// on an SM, or 256 (16-bit operands; e4m3: the wide form, 128 rows on the M side and 256 weights).  By the time that the tiles take in rounds of what is resident, from the
+// measured times of a k-step, in hundredths of a microsecond.  (us, bf16 / e4m3, 32, 64, 128 and 256 rows: 4096 rows, N = 1000,
+// K = 4096 95 55 58 47 / 65 47 38 30; 300 rows 19 16 16 43 / 15 14 14 27; 2000 rows in eight groups, N = 4096, K = 2048 100 58 72 64 /
+// 67 50 50 44; 2000 in 32, N = 1000, K = 4096 75 64 57 63 / 49 45 38 35.)
+int choose_rows(const ProductArgs &a, bool scaled, bool gated, int kblocks, int num_sms) {
+#ifdef OCCAMY_TUNING
+  if (const char *e = getenv("OCCAMY_PT_BN")) return atoi(e);
+#endif
+  static const int rows_of[4] = {32, 64, 128, 256};
+  static const int step[2][4] = {{34, 37, 0, 61}, {45, 60, 47, 58}};
+  const double live = (double)std::min(a.groups, a.rows);
+  int best = 0;
+  double least = 0;
+  for (int i = 0; i < 4; ++i) {
+    if (!scaled && i == 2) continue;
+    const bool wide = scaled && i == 3;
+    const double m = wide ? 128 : rows_of[i], n = (wide ? 256 : PT_ROWS) / (gated ? 2 : 1);
+    const double tiles = std::max(a.groups == 1 ? std::ceil(a.rows / m) : a.rows / m + 0.5 * live, live) * std::ceil(a.N / n);
+    const double slots = (double)num_sms * (i < 2 ? 2 : 1);
+    const int shares = i < 3 ? shares_of_k((int64_t)tiles, (int64_t)slots, kblocks) : 1;
+    const double full = tiles * shares / slots, rounds = std::max(1.0, 0.5 * (full + std::ceil(full)));
+    const double t = rounds * ((kblocks + shares - 1) / shares) * step[scaled][i] + (shares > 1 ? 300 : 0);
+    if (i == 0 || t < least) best = i, least = t;
+  }
+  return rows_of[best];
+}
+
 template <int BN, bool SCALED, bool GATED>
 cudaError_t launch_tiles(PtParams &p, int64_t most_tiles, int num_sms, cudaStream_t s) {
   constexpr size_t LIMIT = BN <= 64 ? TC_SMEM_DUO : TC_SMEM_LIMIT;
@@ -501,11 +533,7 @@ cudaError_t launch_tiles(PtParams &p, int64_t most_tiles, int num_sms, cudaStrea
   const size_t misc = EW * 1024 + (SCALED ? p.bufs * (GATED ? 2 : 1) * BN * 4 : 0) + 8 * 3 * 4 + 16 +
                       (3 * (size_t)p.groups + 1) * 4;
   const size_t stage = (PT_ROWS + BN) * 128 + 16;
-  size_t limit = LIMIT;
-#ifdef OCCAMY_TUNING
-  if (getenv("OCCAMY_PT_SMEM")) limit = TC_SMEM_LIMIT;
-#endif
-  p.stages = (int)std::min<size_t>((limit - misc) / stage, 16);
+  p.stages = (int)std::min<size_t>((LIMIT - misc) / stage, 16);
   const size_t smem = p.stages * stage + misc;
   // the attribute is the device's: set for each once
   static std::once_flag once[64];
@@ -513,37 +541,23 @@ cudaError_t launch_tiles(PtParams &p, int64_t most_tiles, int num_sms, cudaStrea
   cudaError_t e = cudaGetDevice(&dev);
   if (e != cudaSuccess) return e;
   std::call_once(once[dev & 63], [] {
-    cudaFuncSetAttribute(block_product_kernel<BN, SCALED, GATED>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)TC_SMEM_LIMIT);
+    cudaFuncSetAttribute(block_product_kernel<BN, SCALED, GATED>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)LIMIT);
     cudaFuncSetAttribute(block_product_kernel<BN, SCALED, GATED>, cudaFuncAttributePreferredSharedMemoryCarveout, cudaSharedmemCarveoutMaxShared);
   });
   const int64_t resident = (int64_t)num_sms * (BN <= 64 ? 2 : 1);
-  p.splits = 1;
-  if constexpr (BN <= 128)
-    while (p.splits < 8 && most_tiles * p.splits * 2 <= resident && p.kblocks >= p.splits * 8) p.splits *= 2;
+  p.splits = BN <= 128 ? shares_of_k(most_tiles, resident, p.kblocks) : 1;
 #ifdef OCCAMY_TUNING
   if (const char *e = getenv("OCCAMY_PT_SPLITS")) p.splits = atoi(e);
-  if (getenv("OCCAMY_PT_LOG")) {
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3((unsigned)(most_tiles * p.splits)); cfg.blockDim = dim3(PT_THREADS); cfg.dynamicSmemBytes = smem;
-    cudaLaunchAttribute at; at.id = cudaLaunchAttributeClusterDimension; at.val.clusterDim.x = p.splits; at.val.clusterDim.y = at.val.clusterDim.z = 1;
-    cfg.attrs = &at; cfg.numAttrs = 1; int n = -1;
-    cudaOccupancyMaxActiveClusters(&n, block_product_kernel<BN, SCALED, GATED>, &cfg);
-    fprintf(stderr, "BN %d tiles %ld splits %d stages %d smem %zu: %d clusters fit\n", BN, (long)most_tiles, p.splits, p.stages, smem, n);
-  }
 #endif
   const int64_t grid = p.splits > 1 ? most_tiles * p.splits : std::min<int64_t>(most_tiles, resident);
   return launch_after(block_product_kernel<BN, SCALED, GATED>, dim3((unsigned)grid), dim3(PT_THREADS), smem, s,
                       p.splits, p);
 }
 
-template <int BN>
-cudaError_t launch_width(PtParams &p, bool scaled, bool gated, int64_t most_tiles, int num_sms, cudaStream_t s) {
-  if constexpr (BN <= 128)
-    if (scaled)
-      return gated ? launch_tiles<BN, true, true>(p, most_tiles, num_sms, s)
-                   : launch_tiles<BN, true, false>(p, most_tiles, num_sms, s);
-  return gated ? launch_tiles<BN, false, true>(p, most_tiles, num_sms, s)
-               : launch_tiles<BN, false, false>(p, most_tiles, num_sms, s);
+template <int BN, bool SCALED>
+cudaError_t launch_width(PtParams &p, bool gated, int64_t most_tiles, int num_sms, cudaStream_t s) {
+  return gated ? launch_tiles<BN, SCALED, true>(p, most_tiles, num_sms, s)
+               : launch_tiles<BN, SCALED, false>(p, most_tiles, num_sms, s);
 }
 
 }  // namespace
@@ -553,8 +567,9 @@ cudaError_t launch_product(const ProductArgs &a, int num_sms, cudaStream_t s) {
   memset(&p, 0, sizeof(p));
   const bool scaled = a.type == ELEM_E4M3, gated = a.act == ACT_GATED_SILU;
   const int es = elem_size(a.type), bk = 128 / es;
-  const int64_t each = (a.rows + a.groups - 1) / a.groups;
-  const bool wide = scaled && each > 128;
+  p.kblocks = (int)((a.K + bk - 1) / bk);
+  const int BN = choose_rows(a, scaled, gated, p.kblocks, num_sms);
+  const bool wide = scaled && BN == 256;
   p.a = (const uint8_t *)a.a;
   p.a_ld16 = (uint32_t)(a.lda * es / 16);
   p.k_bytes = (int)(a.K * es);
@@ -589,7 +604,6 @@ cudaError_t launch_product(const ProductArgs &a, int num_sms, cudaStream_t s) {
   p.N = (int)a.N;
   p.act = a.act;
   p.out_type = a.out_type;
-  p.kblocks = (int)((a.K + bk - 1) / bk);
   p.blocks_n = (int)scale_blocks(a.N);
   // F32 accumulator; the type of A and B (f16 0, bf16 1, e4m3 0); M = 128
   const uint32_t fmt = a.type == ELEM_BF16 ? 1u : 0u;
@@ -599,18 +613,24 @@ cudaError_t launch_product(const ProductArgs &a, int num_sms, cudaStream_t s) {
 #ifdef OCCAMY_TC_TIMERS
   p.timers = tc_timer_words();
 #endif
-  const int BN = each <= 32 ? 32 : (each <= 64 ? 64 : (each <= 128 ? 128 : 256));
   const int tile_m = wide ? 128 : BN, tile_n = (wide ? 256 : PT_ROWS) / (gated ? 2 : 1);
   p.tiles_n = (int)((a.N + tile_n - 1) / tile_n);
   // (rows of g groups fill at most so many tiles)
   const int64_t most_tiles =
       std::min<int64_t>((a.rows + std::min(a.groups, a.rows) * (tile_m - 1)) / tile_m * p.tiles_n, 1 << 28);
-  if (wide) return launch_product_wide(p, gated, most_tiles, num_sms, s);
+  count((Counter)(CNT_PRODUCT_32 + (BN == 32 ? 0 : BN == 64 ? 1 : BN == 128 ? 2 : 3)));
+  if (scaled) {
+    switch (BN) {
+      case 32: return launch_width<32, true>(p, gated, most_tiles, num_sms, s);
+      case 64: return launch_width<64, true>(p, gated, most_tiles, num_sms, s);
+      case 128: return launch_width<128, true>(p, gated, most_tiles, num_sms, s);
+      default: return launch_product_wide(p, gated, most_tiles, num_sms, s);
+    }
+  }
   switch (BN) {
-    case 32: return launch_width<32>(p, scaled, gated, most_tiles, num_sms, s);
-    case 64: return launch_width<64>(p, scaled, gated, most_tiles, num_sms, s);
-    case 128: return launch_width<128>(p, scaled, gated, most_tiles, num_sms, s);
-    default: return launch_width<256>(p, scaled, gated, most_tiles, num_sms, s);
+    case 32: return launch_width<32, false>(p, gated, most_tiles, num_sms, s);
+    case 64: return launch_width<64, false>(p, gated, most_tiles, num_sms, s);
+    default: return launch_width<256, false>(p, gated, most_tiles, num_sms, s);
   }
 }
 

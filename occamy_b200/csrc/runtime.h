@@ -90,7 +90,8 @@ enum Counter {
   CNT_SUMMED = 14,
   CNT_PAIRS = 15,
   CNT_ROWS = 16,
-  CNT_COUNT = 17
+  CNT_PRODUCT_32 = 17,   // and three more: tiles of 64, 128, 256 rows
+  CNT_COUNT = 21
 };
 
 struct Runtime {

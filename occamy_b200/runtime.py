@@ -173,7 +173,7 @@ def counters() -> dict:
 
 
 FORM_NAMES = ("split_reduction", "inverted_residual", "column_strips", "pooled", "replayed", "in_pieces", "summed",
-              "pairs", "input_rows")
+              "pairs", "input_rows", "product_32", "product_64", "product_128", "product_256")
 
 
 def form_counters() -> dict:

@@ -303,6 +303,86 @@ def test_grouped_larger(type):
     assert torch.equal(out, again)
 
 
+# Sizes that make the calls take each form: tiles of 32, 64, 128 rows, and of 256 (e4m3: 128 rows and 256 weights).
+FORMS = {32: ([3, 0, 30, 33, 1], 264, 520), 64: ([60] * 4 + [0, 130, 64, 65, 7] + [50] * 32, 1032, 264),
+         128: ([512, 0, 130, 257, 3, 128], 1032, 1288), 256: ([300, 0, 1, 1290, 256, 511, 777, 64], 2056, 328)}
+
+
+@pytest.mark.parametrize("rows", list(FORMS))
+@pytest.mark.parametrize("type", ["bf16", "e4m3"])
+@pytest.mark.parametrize("act,out_type,bias", [("gated", "bf16", False), ("gated", "fp32", True), ("none", "fp32", True),
+                                               ("relu", "fp16", True), ("silu", "bf16", False), ("none", "bf16", False)])
+@pytest.mark.parametrize("gathered", [False, True])
+def test_products_in_every_form(rows, type, act, out_type, bias, gathered):
+    sizes, n, k = FORMS[rows]
+    both = (2,) if act == "gated" else ()
+    if act == "gated":
+        n //= 2
+        n -= n % 8
+    gen = generator(rows + k)
+    groups, used = len(sizes), sum(sizes)
+    sources = 200 if gathered else used
+    sa = sb = None
+    if type == "e4m3":
+        a, sa = ec.e4m3(gen, sources, k)
+        b, sb = ec.e4m3(gen, groups, *both, n, k, scale=k ** -0.5, block_rows=128)
+    else:
+        a = ec.rows_apart(torch.randn(sources, k, generator=gen, device="cuda").bfloat16(), 8)
+        b = ec.rows_apart((torch.randn(groups, *both, n, k, generator=gen, device="cuda") * k ** -0.5).bfloat16(), 8)
+    bias = torch.randn(groups, *both, n, generator=gen, device="cuda") if bias else None
+    index = None
+    if gathered:
+        index = torch.randint(0, sources, (used,), generator=gen, device="cuda", dtype=torch.int32)
+        index[5], index[used // 2], index[used - 1] = -1, sources, 2147483647
+    offsets = torch.tensor(list(itertools.accumulate([0] + sizes)), dtype=torch.int32, device="cuda")
+    av = ec.values(a, sa, 1) if sa is not None else a.double()
+    for extra in (8, 3):       # rows of the result at multiples of 16 bytes, and anywhere
+        base, out = kept(used, n, TYPES[out_type], extra=extra)
+        assert ec.grouped(a, offsets, b, out, sa, sb, act, bias, index) == 0
+        for g in range(groups):
+            lo, hi = sum(sizes[:g]), sum(sizes[:g + 1])
+            if lo == hi:
+                continue
+            bv = ec.values(b[g], sb[g], 128) if sb is not None else b[g].double()
+            ar = av[lo:hi]
+            if gathered:
+                i = index[lo:hi].long()
+                there = (i >= 0) & (i < sources)
+                ar = torch.where(there[:, None], av[i.clamp(0, sources - 1)], torch.zeros_like(av[:1]))
+            ec.close(out[lo:hi], *ec.product64(ar, bv, bias[g] if bias is not None else None, act, TYPES[out_type]))
+        assert (base[:, n:].float() == torch.tensor(KEEP).to(TYPES[out_type]).float().item()).all()
+        again = torch.full_like(base, KEEP)[:, :n]
+        assert ec.grouped(a, offsets, b, again, sa, sb, act, bias, index) == 0
+        assert torch.equal(out, again)
+
+
+def test_forms_of_one_group():
+    """The counters say which tiles calls take."""
+    gen = generator(1)
+
+    def one(type, m, n, k):
+        before = rt.form_counters()
+        if type == "e4m3":
+            (a, sa), (b, sb) = ec.e4m3(gen, m, k), ec.e4m3(gen, n, k, scale=k ** -0.5, block_rows=128)
+            out = torch.empty(m, n, dtype=torch.bfloat16, device="cuda")
+            assert ec.matmul(a, sa, b, sb, out) == 0
+            ec.close(out, *ec.product64(ec.values(a, sa, 1), ec.values(b, sb, 128), None, "none", torch.bfloat16))
+        else:
+            a = torch.randn(m, k, generator=gen, device="cuda").to(TYPES[type])
+            b = (torch.randn(1, n, k, generator=gen, device="cuda") * k ** -0.5).to(TYPES[type])
+            out = torch.empty(m, n, dtype=TYPES[type], device="cuda")
+            offsets = torch.tensor([0, m], dtype=torch.int32, device="cuda")
+            assert ec.grouped(a, offsets, b, out) == 0
+            ec.close(out, *ec.product64(a.double(), b[0].double(), None, "none", TYPES[type]))
+        return [f for f, v in rt.form_counters().items() if v != before[f]]
+    assert one("e4m3", 20, 4096, 2048) == ["product_32"]
+    assert one("e4m3", 300, 4096, 2048) == ["product_128"]
+    assert one("e4m3", 2048, 4096, 1024) == ["product_256"]
+    assert one("fp16", 20, 4096, 2048) == ["product_32"]
+    assert one("fp16", 300, 4096, 2048) == ["product_64"]
+    assert one("fp16", 4096, 4096, 256) == ["product_256"]
+
+
 # ------------------------------------------------------------------------------------------- routing
 def route64(logits, k, normalise):
     l = logits.double().cpu().numpy()
