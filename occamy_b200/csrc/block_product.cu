@@ -40,7 +40,7 @@ __global__ void __launch_bounds__(PT_THREADS, BN <= 64 ? 2 : 1) block_product_ke
   constexpr int EW = PT_EPI_WARPS;
   constexpr int CW = BN / (EW / 4);      // columns of an epilogue warp
   constexpr int NG = CW / 8;             // groups of eight of them
-  constexpr int LD = CW == 32 ? 32 : 16;  // columns of one TMEM load (128 sums leave no registers for more)
+  constexpr int LD = CW < 32 ? CW : 32;  // columns of one TMEM load
   constexpr int SETS = GATED ? 2 : 1;    // scales of a column: first and second matrix
   constexpr int TILE_N = GATED ? PT_ROWS / 2 : PT_ROWS;
   extern __shared__ __align__(1024) uint8_t smem_raw[];
@@ -90,7 +90,11 @@ __global__ void __launch_bounds__(PT_THREADS, BN <= 64 ? 2 : 1) block_product_ke
                  : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
   }
-  pt_find_groups<PT_THREADS, BN>(p, groups, lane);
+  pdl_launch_dependents();
+  pdl_wait();
+  pt_read_groups<PT_THREADS>(p, groups);
+  __syncthreads();
+  if (warp == 0) pt_count_tiles<BN>(p, groups, lane);
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
@@ -499,15 +503,15 @@ int shares_of_k(int64_t tiles, int64_t resident, int kblocks) {
 
 // Rows of a tile: 32, 64, 128 (e4m3; with 16 bits two CTAs of 64 were as fast) with the rows on the N side, two CTAs of the first two
 // on an SM, or 256 (16-bit operands; e4m3: the wide form, 128 rows on the M side and 256 weights).  By the time that the tiles take in rounds of what is resident, from the
-// measured times of a k-step, in hundredths of a microsecond.  (us, bf16 / e4m3, 32, 64, 128 and 256 rows: 4096 rows, N = 1000,
-// K = 4096 95 55 58 47 / 65 47 38 30; 300 rows 19 16 16 43 / 15 14 14 27; 2000 rows in eight groups, N = 4096, K = 2048 100 58 72 64 /
-// 67 50 50 44; 2000 in 32, N = 1000, K = 4096 75 64 57 63 / 49 45 38 35.)
+// measured times of a k-step, in hundredths of a microsecond.  (us with 32, 64 and 256 rows in bf16, 32, 64, 128 and 256 in e4m3: 4096
+// rows, N = 1000, K = 4096 63 45 32 and 60 46 37 25; 300 rows 15 14 26 and 15 14 14 22; 2000 rows in eight groups 37 28 33 and 34 26 36 24;
+// 5000 in 32 89 74 66 and 76 64 60 48.)
 int choose_rows(const ProductArgs &a, bool scaled, bool gated, int kblocks, int num_sms) {
 #ifdef OCCAMY_TUNING
   if (const char *e = getenv("OCCAMY_PT_BN")) return atoi(e);
 #endif
   static const int rows_of[4] = {32, 64, 128, 256};
-  static const int step[2][4] = {{34, 37, 0, 61}, {45, 60, 47, 58}};
+  static const int step[2][4] = {{24, 32, 0, 40}, {43, 63, 50, 56}};
   const double live = (double)std::min(a.groups, a.rows);
   int best = 0;
   double least = 0;

@@ -183,28 +183,18 @@ __device__ __forceinline__ void store_row(const PtParams &p, uint8_t *out, const
 struct PtGroups {
   int32_t *first, *last, *before;
 };
-// By all threads, behind which they have to meet; and the point from which on memory that other kernels write is touched.
-// Offsets are cut off at [0, rows].
-template <int THREADS, int ROWS>
-__device__ __forceinline__ void pt_find_groups(const PtParams &p, const PtGroups &t, int lane) {
-  pdl_launch_dependents();
-  if (!p.offsets) {
-    if (threadIdx.x == 0) {
-      t.first[0] = t.before[0] = 0;
-      t.last[0] = p.rows;
-      t.before[1] = (p.rows + ROWS - 1) / ROWS;
-    }
-    pdl_wait();
-    return;
-  }
-  pdl_wait();
+// By all threads; they have to meet before anything is read.  Offsets are cut off at [0, rows].
+template <int THREADS>
+__device__ __forceinline__ void pt_read_groups(const PtParams &p, const PtGroups &t) {
   for (int g = threadIdx.x; g < p.groups; g += THREADS) {
-    const int lo = min(max(p.offsets[g], 0), p.rows);
+    const int lo = p.offsets ? min(max(p.offsets[g], 0), p.rows) : 0;
     t.first[g] = lo;
-    t.last[g] = min(max(p.offsets[g + 1], lo), p.rows);
+    t.last[g] = p.offsets ? min(max(p.offsets[g + 1], lo), p.rows) : p.rows;
   }
-  __syncthreads();
-  if (threadIdx.x >= 32) return;
+}
+// By one warp, behind that.
+template <int ROWS>
+__device__ __forceinline__ void pt_count_tiles(const PtParams &p, const PtGroups &t, int lane) {
   int sum = 0;
   for (int g0 = 0; g0 < p.groups; g0 += 32) {
     const int g = g0 + lane, n = g < p.groups ? (t.last[g] - t.first[g] + ROWS - 1) / ROWS : 0;

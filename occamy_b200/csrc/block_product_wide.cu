@@ -79,7 +79,11 @@ __global__ void __launch_bounds__(PT_THREADS, 1) block_product_wide_kernel(const
                  : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
   }
-  pt_find_groups<PT_THREADS, PW_ROWS>(p, groups, lane);
+  pdl_launch_dependents();
+  pdl_wait();
+  pt_read_groups<PT_THREADS>(p, groups);
+  __syncthreads();
+  if (warp == 0) pt_count_tiles<PW_ROWS>(p, groups, lane);
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
