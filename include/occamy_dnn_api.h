@@ -269,7 +269,8 @@ int64_t occamy_noalloc_capacity(void);
  *   - tensors are row-major; `ld...` is the distance between rows, in elements.  Element types: 0 fp32, 1 bf16, 2 fp16,
  *     3 e4m3 (8-bit floating point, largest value 448, no infinity).
  *   - every pointer is memory of the CURRENT device, results overlap no input, and work is enqueued on `stream`, a stream of
- *     that device; nothing waits and nothing is allocated, so calls can be captured into a graph.  `stream` may be any,
+ *     that device; nothing waits and nothing is allocated, so calls can be captured into a graph, all but the process's first
+ *     (refused with -6; it sets the runtime up).  `stream` may be any,
  *     occamy_stream() among them.  Memory that came from wrapDNNMalloc or a pool is brought up to date first (a result
  *     that a convolution left in another format, for instance) and ordered with the runtime's own stream on both sides;
  *     while `stream` is captured such memory is refused (-6), unless `stream` is occamy_stream().
@@ -296,8 +297,8 @@ int occamy_matmul_e4m3(const void *a, int64_t lda, const float *scaleA, const vo
                        const float *scaleB, const float *bias, int64_t M, int64_t N, int64_t K,
                        int64_t activMode, void *out, int outType, int64_t ldo, cudaStream_t stream);
 /* The same for rows in groups: rows offsets[g] .. offsets[g + 1] - 1 of out are the rows of A times matrix g of B.
- * offsets: groups + 1 numbers in device memory, ascending, cut off at [0, rows]; rows in front of the first and behind the last are
- * left as they were.  Row i is row index[i] of A[aRows][K], one outside [0, aRows) counts as zeros (index null: row i, and rows ==
+ * offsets: groups + 1 numbers in device memory, ascending, cut off at [0, rows] (one below an earlier one counts as that); rows in
+ * front of the first and behind the last are left as they were.  Row i is row index[i] of A[aRows][K], one outside [0, aRows) counts as zeros (index null: row i, and rows ==
  * aRows; with one, A has at most 64 GiB).  type 1 or 2: A and B are bf16 / fp16 and have no scales; type 3: as above, with scaleB [groups][ceil(N / 128)]
  * [ceil(K / 128)].  B: [groups][N][K], rows ldb apart, bias: [groups][N] or null.  Up to 1024 groups.
  * activMode 7: out = silu(first) * second of two matrices for each group; then B is [groups][2][N][K], scaleB and bias have

@@ -107,6 +107,16 @@ __global__ void __launch_bounds__(PT_THREADS, BN <= 64 ? 2 : 1) block_product_ke
   constexpr int PER = SCALED ? 1 : PT_PER;
   int err_code = 0;
   auto decode = [&](int tile) { return pt_decode<BN, TILE_N>(p, groups, tile); };
+  // By all warps.  CTAs of a cluster do it before they wait for each other: one that waited with its columns for a CTA that waits for
+  // columns could do so for good, if what holds those waits in the same way (another kernel's cluster, on another stream).
+  auto free_tmem = [&] {
+    tc_fence_before();
+    __syncthreads();
+    if (warp == 1) {
+      tc_fence_after();
+      asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(COLS) : "memory");
+    }
+  };
 
   // An epilogue warp's place.
   const int ew = warp - PT_EPI_WARP, quad = warp & 3, c0 = (ew >> 2) * CW;
@@ -304,6 +314,7 @@ __global__ void __launch_bounds__(PT_THREADS, BN <= 64 ? 2 : 1) block_product_ke
   }
   if (splits > 1) {   // where the sums' warps meet, the CTAs of the cluster among them
     __syncwarp();
+    free_tmem();
     cluster_sync_all();
   }
   } else {
@@ -430,6 +441,7 @@ __global__ void __launch_bounds__(PT_THREADS, BN <= 64 ? 2 : 1) block_product_ke
         for (int i = 0; i < CW / 2; ++i) sums[i * (EW * 32) + threadIdx.x - 32 * PT_EPI_WARP] = acc[i];
       }
       __syncwarp();
+      free_tmem();
       cluster_sync_all();
       if (mine) {
         const PtTile tl = decode(tile0);
@@ -465,13 +477,8 @@ __global__ void __launch_bounds__(PT_THREADS, BN <= 64 ? 2 : 1) block_product_ke
     *abort_flag = 1;
     if (lane == 0) atomicExch(p.err, 1000 + err_code);
   }
-  tc_fence_before();
-  __syncthreads();
   if (splits > 1) cluster_sync_all();   // nobody leaves while its sums are still to be read
-  if (warp == 1) {
-    tc_fence_after();
-    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(COLS) : "memory");
-  }
+  else free_tmem();
 }
 
 typedef CUresult (*EncodeFn)(CUtensorMap *, CUtensorMapDataType, cuuint32_t, void *, const cuuint64_t *, const cuuint64_t *,

@@ -187,24 +187,38 @@ struct PtGroups {
 template <int THREADS>
 __device__ __forceinline__ void pt_read_groups(const PtParams &p, const PtGroups &t) {
   for (int g = threadIdx.x; g < p.groups; g += THREADS) {
-    const int lo = p.offsets ? min(max(p.offsets[g], 0), p.rows) : 0;
-    t.first[g] = lo;
-    t.last[g] = p.offsets ? min(max(p.offsets[g + 1], lo), p.rows) : p.rows;
+    t.first[g] = p.offsets ? min(max(p.offsets[g], 0), p.rows) : 0;
+    t.last[g] = p.offsets ? min(max(p.offsets[g + 1], 0), p.rows) : p.rows;
   }
 }
-// By one warp, behind that.
+// By one warp, behind that: how many row tiles come before each group.  An offset below one in front of it counts as that one: no
+// row is in two groups, whatever the offsets are.
 template <int ROWS>
 __device__ __forceinline__ void pt_count_tiles(const PtParams &p, const PtGroups &t, int lane) {
-  int sum = 0;
+  int sum = 0, top = t.first[0];
   for (int g0 = 0; g0 < p.groups; g0 += 32) {
-    const int g = g0 + lane, n = g < p.groups ? (t.last[g] - t.first[g] + ROWS - 1) / ROWS : 0;
+    const int g = g0 + lane;
+    int end = g < p.groups ? max(t.last[g], top) : top;
+#pragma unroll
+    for (int d = 1; d < 32; d *= 2) {
+      const int o = __shfl_up_sync(0xffffffffu, end, d);
+      if (lane >= d) end = max(end, o);
+    }
+    int begin = __shfl_up_sync(0xffffffffu, end, 1);
+    if (lane == 0) begin = top;
+    top = __shfl_sync(0xffffffffu, end, 31);
+    const int n = g < p.groups ? (end - begin + ROWS - 1) / ROWS : 0;
     int upto = n;
 #pragma unroll
     for (int d = 1; d < 32; d *= 2) {
       const int o = __shfl_up_sync(0xffffffffu, upto, d);
       if (lane >= d) upto += o;
     }
-    if (g < p.groups) t.before[g] = sum + upto - n;
+    if (g < p.groups) {
+      t.first[g] = begin;
+      t.last[g] = end;
+      t.before[g] = sum + upto - n;
+    }
     sum += __shfl_sync(0xffffffffu, upto, 31);
   }
   if (lane == 0) t.before[p.groups] = sum;

@@ -54,6 +54,13 @@ class Call {
         return refuse(NO_DEVICE, who_, "cannot read the number of SMs");
     }
     num_sms_ = sms[device_];
+    // the runtime's state is set up by the first call of any kind, which a stream that is captured does not allow
+    static bool ready = false;
+    if (!ready) {
+      if (capturing()) return refuse(CAPTURED, who_, "the first call cannot be captured");
+      rt();
+      ready = true;
+    }
     if (stream_ == rt().stream) {
       occamy_internal_opaque_call();
       settled_ = true;
@@ -94,13 +101,8 @@ class Call {
     if (at.type != cudaMemoryTypeManaged && (at.type != cudaMemoryTypeDevice || at.device != device_))
       return refuse(BAD_POINTER, who_, "an address is not memory of the current device");
     if (!reg_find(p)) return 0;
-    if (stream_ != rt().stream) {
-      cudaStreamCaptureStatus st = cudaStreamCaptureStatusNone;
-      if (cudaStreamIsCapturing(stream_, &st) != cudaSuccess || st != cudaStreamCaptureStatusNone) {
-        cudaGetLastError();
-        return refuse(CAPTURED, who_, "memory of the runtime's own cannot be used while the stream is captured");
-      }
-    }
+    if (stream_ != rt().stream && capturing())
+      return refuse(CAPTURED, who_, "memory of the runtime's own cannot be used while the stream is captured");
     if (!settled_) {
       occamy_internal_opaque_call();
       settled_ = true;
@@ -109,6 +111,12 @@ class Call {
     ensure_f32(p);   // a result may leave parts of its memory as they were: they have to be there too
     if (written) mark_f32(const_cast<void *>(p));
     return 0;
+  }
+  bool capturing() const {
+    cudaStreamCaptureStatus st = cudaStreamCaptureStatusNone;
+    if (cudaStreamIsCapturing(stream_, &st) == cudaSuccess && st == cudaStreamCaptureStatusNone) return false;
+    cudaGetLastError();
+    return true;
   }
   int order(cudaStream_t first, cudaStream_t then) {
     cudaEvent_t ev;

@@ -5,7 +5,8 @@
 Every row calls one ABI symbol (pooling, element-wise add / ReLU / Clip, depthwise convolution,
 global average pool, softmax) on device-resident tensors of the sizes ResNet-50 and MobileNetV2
 produce at the given batch, in bf16 mode with the input already in the runtime's bf16 NHWC
-format (it is the output of a convolution call, as in a model).  Times are CUDA-event medians on
+format (it is the output of a convolution call, as in a model).  Single convolution layers and the 8-bit and
+grouped operators (`--only e4m3,grouped,route,combine`) are timed when they are named.  Times are CUDA-event medians on
 the runtime's stream; between repetitions the tensors (hundreds of MB) do not fit the L2.
 "achieved" is algorithmic bytes / time, "frac" its share of the measured copy bandwidth in
 MEASURED_PEAKS.json (fallback 6650 GB/s).
@@ -169,6 +170,7 @@ def run(batch=256, reps=20, only="", math=rt.MATH_BF16, role_timers=False):
     _rest(h, rng, B, L, timed, depthwise, sel)
     if any("conv" in t for t in wanted):
         _conv_rows(h, rng, B, L, timed, wanted)
+    _expert_rows(rng, B, L, timed, wanted)
     L.cudnnDestroy(h)
     return rows, peak, peak_src
 
@@ -252,6 +254,69 @@ def _conv_rows(h, rng, B, L, timed, wanted):
         timed(f"{name} [{B}] ({flops / 1e9:.1f} GFLOP)", nbytes, call)
         for t in (x, w, b, y):
             t.buf.free()
+
+
+def _ok(code):
+    if code:
+        raise SystemExit(f"refused: {code}")
+
+
+def _expert_rows(rng, B, L, timed, wanted):
+    """The 8-bit and grouped operators; timed only when named in `only` ("e4m3", "grouped", "route", "combine").  VGG-16's first
+    classifier layer at the given batch; an expert layer with 32 experts, 4 for each of 16 B tokens."""
+    s = L.occamy_stream()
+
+    def bytes_(n, random=False):
+        if not random:
+            return rt.DeviceBuffer(n)
+        return rt.DeviceBuffer.from_numpy(rng.integers(0, 120, n, dtype=np.uint8))   # e4m3 numbers up to 240
+
+    def on(*pieces):
+        return any(any(t in p for p in pieces) for t in wanted)
+    n, k = 4096, 25088
+    if on("quantise e4m3 weights", "e4m3"):
+        w, q, qs = _T((n, k), rng.standard_normal((n, k), dtype=np.float32)), bytes_(n * k), bytes_(n * k // 4096)
+        timed(f"quantise e4m3 weights [{n},{k}] fp32", 5 * n * k,
+              lambda: _ok(L.occamy_quantize_e4m3(w.ptr, rt.F32, n, k, k, None, n, 128, q.ptr, k, qs.ptr, s)))
+        w.buf.free(), q.free(), qs.free()
+    if on("product e4m3", "e4m3"):
+        a, b, sa, sb = bytes_(B * k, True), bytes_(n * k, True), bytes_(B * k // 32), bytes_(n * k // 4096)
+        out = bytes_(2 * B * n)
+        timed(f"product e4m3 [{B},{k}] x [{n},{k}] ({2e-9 * B * n * k:.1f} GFLOP)", (B + n) * k + 2 * B * n,
+              lambda: _ok(L.occamy_matmul_e4m3(a.ptr, k, sa.ptr, b.ptr, k, sb.ptr, None, B, n, k, 1, out.ptr, rt.BF16, n, s)))
+        for t in (a, b, sa, sb, out):
+            t.free()
+    if not on("grouped e4m3", "grouped bf16", "route", "combine", "quantise e4m3 rows", "e4m3"):
+        return
+    tokens, experts, c, hidden, inner = 16 * B, 32, 4, 2048, 1024
+    rows = tokens * c
+    logits = _T((tokens, experts), rng.standard_normal((tokens, experts), dtype=np.float32))
+    chosen, weights, position, order = (bytes_(4 * rows) for _ in range(4))
+    offsets, need = bytes_(4 * (experts + 1)), L.occamy_route_experts_workspace(tokens, experts, c)
+    work = bytes_(max(need, 4))
+
+    def route():
+        _ok(L.occamy_route_experts(logits.ptr, rt.F32, tokens, experts, experts, c, 1, chosen.ptr, weights.ptr, offsets.ptr,
+                                   order.ptr, position.ptr, work.ptr, need, s))
+    route()
+    timed(f"route [{tokens},{experts}], {c} each", 4 * tokens * experts + 16 * rows, route)
+    x, q, qs = bytes_(2 * tokens * hidden), bytes_(rows * hidden), bytes_(rows * hidden // 32)
+    timed(f"quantise e4m3 rows [{tokens},{hidden}] bf16 -> {rows}", 2 * tokens * hidden + rows * hidden,
+          lambda: _ok(L.occamy_quantize_e4m3(x.ptr, rt.BF16, tokens, hidden, hidden, order.ptr, rows, 1, q.ptr, hidden, qs.ptr, s)))
+    y = bytes_(2 * rows * inner)
+    for name, code, size in (("e4m3", rt.E4M3, 1), ("bf16", rt.BF16, 2)):
+        b, sb = bytes_(experts * 2 * inner * hidden * size), bytes_(experts * 2 * inner * hidden // 4096)
+        flops = 4.0 * rows * inner * hidden
+        timed(f"grouped {name}, gated, {rows} rows, {experts} x [{inner},{hidden}] ({flops / 1e9:.1f} GFLOP)",
+              (rows + experts * 2 * inner) * hidden * size + 2 * rows * inner,
+              lambda: _ok(L.occamy_matmul_grouped(q.ptr if size == 1 else x.ptr, code, rows if size == 1 else tokens, hidden,
+                                                  qs.ptr, None if size == 1 else order.ptr, offsets.ptr, experts, b.ptr, hidden,
+                                                  sb.ptr, None, rows, inner, hidden, rt.ACT_GATED_SILU, y.ptr, rt.BF16, inner, s)))
+        b.free(), sb.free()
+    out = bytes_(2 * tokens * inner)
+    timed(f"combine [{rows},{inner}] bf16 -> {tokens}", 2 * (rows + tokens) * inner,
+          lambda: _ok(L.occamy_combine_experts(y.ptr, rt.BF16, rows, inner, position.ptr, weights.ptr, tokens, c, inner, out.ptr,
+                                               rt.BF16, inner, s)))
 
 
 def _rest(h, rng, B, L, timed, depthwise, sel):

@@ -274,6 +274,35 @@ def test_grouped_offsets_beyond_the_rows_are_cut_off(type):
     del guard
 
 
+@pytest.mark.parametrize("type", ["bf16", "e4m3"])
+@pytest.mark.parametrize("rows", [70, 3000])
+def test_grouped_offsets_that_go_back(type, rows):
+    """An offset below an earlier one counts as that one: no row is in two groups, and none outside is written."""
+    gen = generator(13)
+    n, k, scale = 1032, 144, rows // 70
+    offsets = [10 * scale, 40 * scale, 5, 30, 60 * scale, -7, 60 * scale]
+    cut, top = [], 0
+    for o in offsets:
+        top = max(top, min(max(o, 0), rows))
+        cut.append(top)
+    groups = len(offsets) - 1
+    if type == "e4m3":
+        a, sa = ec.e4m3(gen, rows, k)
+        b, sb = ec.e4m3(gen, groups, n, k, block_rows=128)
+    else:
+        a, b, sa, sb = (torch.randn(rows, k, generator=gen, device="cuda").bfloat16(),
+                        torch.randn(groups, n, k, generator=gen, device="cuda").bfloat16(), None, None)
+    base, out = kept(rows, n, torch.float32, extra=8)
+    assert ec.grouped(a, torch.tensor(offsets, dtype=torch.int32, device="cuda"), b, out, sa, sb) == 0
+    av = ec.values(a, sa, 1) if sa is not None else a.double()
+    for g in range(groups):
+        lo, hi = cut[g], cut[g + 1]
+        if lo < hi:
+            bv = ec.values(b[g], sb[g], 128) if sb is not None else b[g].double()
+            ec.close(out[lo:hi], *ec.product64(av[lo:hi], bv, None, "none", torch.float32))
+    assert (base[:cut[0]] == KEEP).all() and (base[cut[-1]:] == KEEP).all() and (base[:, n:] == KEEP).all()
+
+
 @pytest.mark.parametrize("type", ["bf16", "fp16", "e4m3"])
 def test_grouped_larger(type):
     """Several tiles of every kind: 1 to 1500 rows a group, gated, gathered."""
@@ -616,6 +645,55 @@ def test_calls_on_a_stream_of_their_own():
         layer(x, l)
     s.synchronize()
     layer.check(x0, l0)
+
+
+def test_the_first_call_is_not_captured():
+    """In a process of its own: the call that sets the runtime up is refused while its stream is captured, and the capture goes on."""
+    import os
+    import subprocess
+    import sys
+    code = (
+        "import torch, expert_calls as ec\n"
+        "x = torch.randn(4, 128, device='cuda'); q = torch.zeros(4, 128, dtype=torch.uint8, device='cuda').view(torch.float8_e4m3fn)\n"
+        "s = torch.zeros(4, 1, device='cuda'); n = torch.zeros(1, device='cuda')\n"
+        "g = torch.cuda.CUDAGraph()\n"
+        "with torch.cuda.graph(g):\n"
+        "    n.add_(1)\n"
+        "    first = ec.quantize(x, q, s)\n"
+        "g.replay(); torch.cuda.synchronize()\n"
+        "assert first == -6 and n.item() == 1 and (s == 0).all(), (first, n.item())\n"
+        "assert ec.quantize(x, q, s) == 0\n"
+        "torch.cuda.synchronize(); assert (s > 0).all()\n"
+        "g = torch.cuda.CUDAGraph(); s.zero_()\n"
+        "with torch.cuda.graph(g):\n"
+        "    assert ec.quantize(x, q, s) == 0\n"
+        "g.replay(); torch.cuda.synchronize(); assert (s > 0).all()\n")
+    here = os.path.dirname(os.path.abspath(__file__))
+    env = {**os.environ, "PYTHONPATH": os.pathsep.join([here, os.path.dirname(here)])}
+    r = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, env=env, timeout=120)
+    assert r.returncode == 0, r.stderr
+
+
+def test_clusters_of_two_streams():
+    """Calls whose tiles are shared by clusters, on two streams at a time."""
+    gen = generator(21)
+    calls = []
+    for m, n, k in ((1, 4096, 4096), (40, 4096, 4096), (90, 2048, 8192), (3, 1000, 4096)):
+        (a, sa), (b, sb) = ec.e4m3(gen, m, k), ec.e4m3(gen, n, k, scale=k ** -0.5, block_rows=128)
+        out = torch.empty(m, n, device="cuda")
+        assert ec.matmul(a, sa, b, sb, out) == 0
+        torch.cuda.synchronize()
+        ec.close(out, *ec.product64(ec.values(a, sa, 1), ec.values(b, sb, 128), None, "none", torch.float32))
+        calls.append((a, sa, b, sb, out.clone(), [torch.empty_like(out) for _ in range(2)]))
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    for _ in range(30):
+        for i, s in enumerate(streams):
+            with torch.cuda.stream(s):
+                for a, sa, b, sb, _, outs in (calls if i else calls[::-1]):
+                    assert ec.matmul(a, sa, b, sb, outs[i]) == 0
+    torch.cuda.synchronize()
+    for *_, want, outs in calls:
+        assert torch.equal(outs[0], want) and torch.equal(outs[1], want)
 
 
 def test_two_threads():
