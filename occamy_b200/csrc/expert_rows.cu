@@ -21,6 +21,11 @@ inline int64_t tokens_of_block(int64_t tokens) {
   return even > RT_TOKENS ? even : RT_TOKENS;
 }
 
+__device__ __forceinline__ float load_logit(const void *p, int64_t i, int type) {
+  if (type == ELEM_F32) return ((const float *)p)[i];
+  if (type == ELEM_BF16) return __bfloat162float(((const __nv_bfloat16 *)p)[i]);
+  return __half2float(((const __half *)p)[i]);
+}
 // Unsigned keys in the order of the values; both zeros alike, every NaN above everything.
 __device__ __forceinline__ uint32_t key_of(float v) {
   if (v != v) return 0xffffffffu;
@@ -57,82 +62,136 @@ __device__ __forceinline__ float warp_sum(float v) {
   return v;
 }
 
-// The k largest logits of token t, by one warp; lane j gets the j-th choice.  V = ceil(experts / 32), the numbers of a lane.
-//
-// 16-bit logits: a lane sorts its words, so that a choice looks at the first of each lane alone: one warp maximum, and the lane that had
-// it moves on (16384 tokens, 128 experts, k = 8: 20 us with all words looked at for every choice, this way PLACEHOLDER).  fp32: the
-// lanes look through theirs, and the lowest expert among equals comes from a second warp minimum.
+// ---- up to eight choices of up to 256 experts (fp32: 128): eight lanes a token
+// A lane holds V neighbouring experts' keys, each with its expert in the low half, so that no two are alike, and sorts them. A choice
+// then looks at the first of each lane alone: three exchanges for the largest, and the lane that had it moves on.  With a token for a
+// whole warp the instructions were few lanes' work: 460 a token, 16384 tokens of 128 experts, k = 8, 17 us; this way 11.
+template <typename T>
+struct KeyOf {   // 16-bit logits
+  typedef uint32_t type;
+  static constexpr type NONE = WORD_NONE<T>;
+  static __device__ __forceinline__ type make(T v, int e) { return word_of(v, e); }
+  static __device__ __forceinline__ float value(type k) { return value_of_word<T>(k); }
+  static __device__ __forceinline__ int expert(type k) { return (int)(0xffffu - (k & 0xffffu)); }
+};
+template <>
+struct KeyOf<float> {
+  typedef unsigned long long type;
+  static constexpr type NONE = (type)KEY_NONE << 32 | 0xffffffffu;
+  static __device__ __forceinline__ type make(float v, int e) { return (type)key_of(v) << 32 | (0xffffffffu - (uint32_t)e); }
+  static __device__ __forceinline__ float value(type k) { return value_of((uint32_t)(k >> 32)); }
+  static __device__ __forceinline__ int expert(type k) { return (int)(0xffffffffu - (uint32_t)k); }
+};
+// Batcher's odd-even merge sort of V = 2^n values, largest first.
+template <int V, typename K>
+__device__ __forceinline__ void sort_down(K *key) {
+#pragma unroll
+  for (int p = 1; p < V; p *= 2)
+#pragma unroll
+    for (int k = p; k >= 1; k /= 2)
+#pragma unroll
+      for (int i = 0; i + k < V; ++i) {
+        // i and i + k, where i is in the first half of its run of 2 k, counted from k % p, and both in the same run of 2 p
+        const int from = i - k % p;
+        if (from >= 0 && from / k % 2 == 0 && i / (2 * p) == (i + k) / (2 * p)) {
+          const K hi = max(key[i], key[i + k]), lo = min(key[i], key[i + k]);
+          key[i] = hi;
+          key[i + k] = lo;
+        }
+      }
+}
+constexpr int EIGHT = 8;
 template <typename T, int V>
-__device__ __forceinline__ void choose(const RouteArgs &a, int64_t t, int lane) {
-  constexpr bool WORDS = sizeof(T) == 2;
-  const T *logits = (const T *)a.logits + t * a.ldl;
-  uint32_t key[V];
+__device__ __forceinline__ void choose_by_eight(const RouteArgs &a, int64_t t0, int64_t t1) {
+  typedef KeyOf<T> Key;
+  typedef typename Key::type K;
+  const int l = threadIdx.x % EIGHT;
+  // (all lanes of a warp go round together: the exchanges are theirs)
+  for (int64_t w = t0 + threadIdx.x / 32 * 4; w < t1; w += RT_THREADS / EIGHT) {
+    const int64_t t = w + (threadIdx.x % 32) / EIGHT;
+    const bool in = t < t1;
+    const T *logits = (const T *)a.logits + t * a.ldl;
+    K key[V];
 #pragma unroll
-  for (int v = 0; v < V; ++v) {
-    const int e = v * 32 + lane;
-    if constexpr (WORDS) key[v] = e < a.experts ? word_of(logits[e], e) : 0u;
-    else key[v] = e < a.experts ? key_of(logits[e]) : 0u;
-  }
-  auto value = [](uint32_t k) {
-    if constexpr (WORDS) return value_of_word<T>(k);
-    else return value_of(k);
-  };
-  constexpr uint32_t none = WORDS ? WORD_NONE<T> : KEY_NONE;
-  uint32_t mine = 0;
-  int expert = -1;
-  float top = 0.0f, total = 0.0f;
-  auto sum_all = [&] {   // behind the first choice
-    float sum = 0.0f;
+    for (int v = 0; v < V; ++v) {
+      const int e = l * V + v;
+      key[v] = in && e < a.experts ? Key::make(logits[e], e) : 0;
+    }
+    float top = 0.0f, total = 0.0f;
+    if (!a.normalise) {
+      K m = 0;
 #pragma unroll
-    for (int v = 0; v < V; ++v)
-      if (key[v] > none) sum += expf(value(key[v]) - top);
-    total = warp_sum(sum);
-  };
-  if constexpr (WORDS && V <= 8) {
-    // odd-even transposition: V rounds
+      for (int v = 0; v < V; ++v) m = max(m, key[v]);
 #pragma unroll
-    for (int r = 0; r < V; ++r)
+      for (int d = EIGHT / 2; d; d /= 2) m = max(m, __shfl_xor_sync(0xffffffffu, m, d));
+      top = Key::value(m);
 #pragma unroll
-      for (int v = r & 1; v + 1 < V; v += 2) {
-        const uint32_t hi = max(key[v], key[v + 1]), lo = min(key[v], key[v + 1]);
-        key[v] = hi;
-        key[v + 1] = lo;
-      }
+      for (int v = 0; v < V; ++v)
+        if (key[v] > Key::NONE) total += expf(Key::value(key[v]) - top);
+    }
+    sort_down<V>(key);
+    K mine = 0;
     for (int j = 0; j < a.k; ++j) {
-      const uint32_t high = __reduce_max_sync(0xffffffffu, key[0]);
-      if (high <= none) break;
-      if (j == 0) {
-        top = value(high);
-        if (!a.normalise) sum_all();
-      }
-      if (lane == j) mine = high, expert = (int)(0xffffu - (high & 0xffffu));
-      if (key[0] == high) {
+      K m = key[0];
+#pragma unroll
+      for (int d = EIGHT / 2; d; d /= 2) m = max(m, __shfl_xor_sync(0xffffffffu, m, d));
+      if (j == 0) top = Key::value(m);
+      if (l == j) mine = m;
+      if (key[0] == m) {
 #pragma unroll
         for (int v = 0; v + 1 < V; ++v) key[v] = key[v + 1];
         key[V - 1] = 0;
       }
     }
-  } else {
-    for (int j = 0; j < a.k; ++j) {
-      uint32_t best = 0;
-      int at = 0;
+    const bool taken = mine > Key::NONE;
+    float p = taken ? expf(Key::value(mine) - top) : 0.0f;
+    if (a.normalise) total = p;
 #pragma unroll
-      for (int v = 0; v < V; ++v)
-        if (key[v] > best) best = key[v], at = v * 32 + lane;
-      const uint32_t high = __reduce_max_sync(0xffffffffu, best);
-      if (high <= none) break;
-      const int e = (int)__reduce_min_sync(0xffffffffu, best == high ? (uint32_t)at : 0xffffffffu);
-      if (j == 0) {
-        top = value(high);
-        if (!a.normalise) sum_all();
-      }
-      if (lane == j) mine = high, expert = e;
-#pragma unroll
-      for (int v = 0; v < V; ++v)
-        if (e == v * 32 + lane) key[v] = 0;
+    for (int d = EIGHT / 2; d; d /= 2) total += __shfl_xor_sync(0xffffffffu, total, d);
+    if (in && l < a.k) {
+      a.chosen[t * a.k + l] = taken ? Key::expert(mine) : -1;
+      a.weights[t * a.k + l] = taken ? p / total : 0.0f;
     }
   }
-  float w = expert >= 0 ? expf(value(mine) - top) : 0.0f;
+}
+
+// ---- any other number of them: a warp a token, lane j gets the j-th choice.  V = ceil(experts / 32), the numbers of a lane.
+template <int V>
+__device__ __forceinline__ void choose(const RouteArgs &a, int64_t t, int lane) {
+  uint32_t key[V];
+#pragma unroll
+  for (int v = 0; v < V; ++v) {
+    const int e = v * 32 + lane;
+    key[v] = e < a.experts ? key_of(load_logit(a.logits, t * a.ldl + e, a.type)) : 0u;
+  }
+  uint32_t mine = 0;
+  int expert = -1;
+  float top = 0.0f, total = 0.0f;
+  for (int j = 0; j < a.k; ++j) {
+    uint32_t best = 0;
+    int at = 0;
+#pragma unroll
+    for (int v = 0; v < V; ++v)
+      if (key[v] > best) best = key[v], at = v * 32 + lane;
+    const uint32_t high = __reduce_max_sync(0xffffffffu, best);
+    if (high <= KEY_NONE) break;
+    const int e = (int)__reduce_min_sync(0xffffffffu, best == high ? (uint32_t)at : 0xffffffffu);
+    if (j == 0) {
+      top = value_of(high);
+      if (!a.normalise) {
+        float sum = 0.0f;
+#pragma unroll
+        for (int v = 0; v < V; ++v)
+          if (key[v] > KEY_NONE) sum += expf(value_of(key[v]) - top);
+        total = warp_sum(sum);
+      }
+    }
+    if (lane == j) mine = high, expert = e;
+#pragma unroll
+    for (int v = 0; v < V; ++v)
+      if (e == v * 32 + lane) key[v] = 0;
+  }
+  float w = expert >= 0 ? expf(value_of(mine) - top) : 0.0f;
   if (a.normalise) total = warp_sum(w);
   if (expert >= 0) w /= total;
   if (lane < a.k) {
@@ -141,9 +200,13 @@ __device__ __forceinline__ void choose(const RouteArgs &a, int64_t t, int lane) 
   }
 }
 
+// V: the numbers of a lane; negative: of eight lanes a token.
 template <typename T, int V>
 __device__ __forceinline__ void choose_block(const RouteArgs &a, int64_t t0, int64_t t1) {
-  for (int64_t t = t0 + (threadIdx.x >> 5); t < t1; t += RT_WARPS) choose<T, V>(a, t, threadIdx.x & 31);
+  if constexpr (V < 0)
+    choose_by_eight<T, -V>(a, t0, t1);
+  else
+    for (int64_t t = t0 + (threadIdx.x >> 5); t < t1; t += RT_WARPS) choose<V>(a, t, threadIdx.x & 31);
 }
 
 // Exclusive prefix sums of one number for each thread; `sums`: 32 words of shared memory.  The last thread's result and number
@@ -313,11 +376,15 @@ cudaError_t launch_route_of(const RouteArgs &a, cudaStream_t s) {
 
 template <typename T>
 cudaError_t launch_route_typed(const RouteArgs &a, cudaStream_t s) {
-  if (a.experts <= 32) return launch_route_of<T, 1>(a, s);
-  if (a.experts <= 64) return launch_route_of<T, 2>(a, s);
-  if (a.experts <= 128) return launch_route_of<T, 4>(a, s);
-  if (a.experts <= 256) return launch_route_of<T, 8>(a, s);
-  return launch_route_of<T, 32>(a, s);
+  if (a.k <= EIGHT) {
+    if (a.experts <= 32) return launch_route_of<T, -4>(a, s);
+    if (a.experts <= 64) return launch_route_of<T, -8>(a, s);
+    if (a.experts <= 128) return launch_route_of<T, -16>(a, s);
+    if constexpr (sizeof(T) == 2)
+      if (a.experts <= 256) return launch_route_of<T, -32>(a, s);
+  }
+  if (a.experts <= 256) return launch_route_of<float, 8>(a, s);
+  return launch_route_of<float, 32>(a, s);
 }
 
 // ---------------------------------------------------------------- weighted sum

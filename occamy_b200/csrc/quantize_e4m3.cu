@@ -79,7 +79,7 @@ struct Eight {
 // 16-byte loads (VEC), else every eighth.  A pass of a CTA covers 2^lanes_log blocks of 32 >> lanes_log rows; a thread keeps its
 // place in the row and goes from row to row, the next one's elements on their way while it works on these.
 // WHOLE: VEC and no block is cut off.  What bounds it is instructions: with eight elements a thread and everything computed anew for each
-// row 64 % of the issue slots (16384 gathered rows of 4096 bf16: 55 us, this way PLACEHOLDER).
+// row 64 % of the issue slots (16384 gathered rows of 4096 bf16: 55 us, this way 32).
 constexpr int QR_LANES = 8;
 template <typename T, bool VEC, bool WHOLE>
 __global__ void __launch_bounds__(256, sizeof(T) == 4 ? 4 : 5) quantize_rows_kernel(QuantArgs a, int blocks, int lanes_log) {
