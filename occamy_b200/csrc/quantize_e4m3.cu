@@ -8,6 +8,8 @@
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
+#include <type_traits>
+
 #include "expert_ops.h"
 #include "kernels.h"
 
@@ -73,25 +75,71 @@ struct Eight {
 #pragma unroll
     for (int j = 0; j < 8; ++j) v[j] = to_float(e[j]);
   }
+  __device__ __forceinline__ void nan_unless_finite() {
+    T *e = reinterpret_cast<T *>(w);
+#pragma unroll
+    for (int j = 0; j < 8; ++j)
+      if (!finite(to_float(e[j]))) e[j] = (T)__int_as_float(0x7fffffff);
+  }
+  // The largest magnitude, NaN passed over; 16-bit types two at a time.
+  static __device__ __forceinline__ float largest(const Eight *e, int n) {
+    if constexpr (sizeof(T) == 4) {
+      float amax = 0.0f;
+#pragma unroll
+      for (int i = 0; i < n; ++i) {
+        float v[8];
+        e[i].values(v);
+        amax = max_of<8>(v, amax);
+      }
+      return amax;
+    } else {
+      using T2 = std::conditional_t<std::is_same_v<T, __half>, __half2, __nv_bfloat162>;
+      T2 m = __habs2(reinterpret_cast<const T2 *>(e[0].w)[0]);
+#pragma unroll
+      for (int i = 0; i < 4 * n; ++i)
+        if (i) m = __hmax2(m, __habs2(reinterpret_cast<const T2 *>(e[i >> 2].w)[i & 3]));
+      return fmaxf(fmaxf(to_float(m.x), to_float(m.y)), 0.0f);   // (of nothing but NaN: 0)
+    }
+  }
+  // In e4m3, times a power of two that leaves no magnitude above 448.  In bf16 that product is exact down to 2^-126, far below what
+  // e4m3 tells from 0 (2^-10), and takes two elements at a time.  (fp16 does not hold all the powers.)
+  __device__ __forceinline__ uint2 packed(float inv) const {
+    float v[8];
+    if constexpr (std::is_same_v<T, __nv_bfloat16>) {
+      const __nv_bfloat162 by = __float2bfloat162_rn(inv);
+      Eight scaled;
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        reinterpret_cast<__nv_bfloat162 *>(scaled.w)[j] = __hmul2(reinterpret_cast<const __nv_bfloat162 *>(w)[j], by);
+      scaled.values(v);
+      inv = 1.0f;
+    } else {
+      values(v);
+    }
+    return make_uint2(pack4(v, inv), pack4(v + 4, inv));
+  }
 };
 
-// Eight threads for each block of 128 elements of a row, sixteen elements for each: two runs of eight, 64 apart, when rows allow
-// 16-byte loads (VEC), else every eighth.  A pass of a CTA covers 2^lanes_log blocks of 32 >> lanes_log rows; a thread keeps its
-// place in the row and goes from row to row, the next one's elements on their way while it works on these.
-// WHOLE: VEC and no block is cut off.  What bounds it is instructions: with eight elements a thread and everything computed anew for each
-// row 64 % of the issue slots (16384 gathered rows of 4096 bf16: 55 us, this way 32).
-constexpr int QR_LANES = 8;
+// A few threads for each block of 128 elements of a row: four of 32 elements (fp32: eight of sixteen) in runs of eight when rows
+// allow 16-byte loads (VEC), else every fourth (eighth) element.  A pass of a CTA covers 2^lanes_log blocks of some rows; a thread
+// keeps its place in the row and goes from row to row, the next one's elements on their way while it works on these.
+// WHOLE: VEC and no block is cut off.  What bounds it is the first-level cache (77 %: lines come in halves) and instructions (61 % of the
+// issue slots): 16384 gathered rows of 4096 bf16 27 us, eight threads a block with all arithmetic in 32 bits 31, without the next
+// row on its way and two CTAs more on an SM 29.
+template <typename T>
+constexpr int QR_LANES = sizeof(T) == 4 ? 8 : 4;
 template <typename T, bool VEC, bool WHOLE>
-__global__ void __launch_bounds__(256, sizeof(T) == 4 ? 4 : 5) quantize_rows_kernel(QuantArgs a, int blocks, int lanes_log) {
+__global__ void __launch_bounds__(256, 4) quantize_rows_kernel(QuantArgs a, int blocks, int lanes_log) {
   chain_begin();
-  const int t = threadIdx.x % QR_LANES, unit = threadIdx.x / QR_LANES;
+  constexpr int LANES = QR_LANES<T>, RUNS = SCALE_BLOCK / (8 * LANES), RUN = 8 * LANES;
+  const int t = threadIdx.x % LANES, unit = threadIdx.x / LANES;
   const int block = (blockIdx.x << lanes_log) + (unit & ((1 << lanes_log) - 1));
-  const int rows_pass = (256 / QR_LANES) >> lanes_log;
+  const int rows_pass = (256 / LANES) >> lanes_log;
   const int left = (int)min((int64_t)SCALE_BLOCK, a.cols - (int64_t)block * SCALE_BLOCK);   // elements of the block
   const T *x = (const T *)a.x + (int64_t)block * SCALE_BLOCK;
   const int64_t step = (int64_t)gridDim.y * rows_pass;
   const int rows = (int)a.rows, x_rows = (int)a.x_rows;
-  auto column = [&](int j) { return VEC ? (j >> 3) * 64 + t * 8 + (j & 7) : t + QR_LANES * j; };
+  auto column = [&](int j) { return VEC ? (j >> 3) * RUN + t * 8 + (j & 7) : t + LANES * j; };
   auto source = [&](int64_t row) {   // -1: none
     if (row >= rows || left <= 0) return -1;
     const int from = a.index ? __ldg(a.index + row) : (int)row;
@@ -101,14 +149,14 @@ __global__ void __launch_bounds__(256, sizeof(T) == 4 ? 4 : 5) quantize_rows_ker
     if (from < 0) return;
     const T *p = x + (int64_t)from * a.ldx;
     if (WHOLE || (VEC && left == SCALE_BLOCK)) {
-      e[0].template load<false>(p + t * 8);
-      e[1].template load<false>(p + 64 + t * 8);
+#pragma unroll
+      for (int i = 0; i < RUNS; ++i) e[i].template load<false>(p + i * RUN + t * 8);
     } else {
-      e[0].clear();
-      e[1].clear();
+#pragma unroll
+      for (int i = 0; i < RUNS; ++i) e[i].clear();
       T *w = reinterpret_cast<T *>(e[0].w);
 #pragma unroll
-      for (int j = 0; j < 16; ++j)
+      for (int j = 0; j < RUNS * 8; ++j)
         if (column(j) < left) w[j] = p[column(j)];
     }
   };
@@ -116,38 +164,43 @@ __global__ void __launch_bounds__(256, sizeof(T) == 4 ? 4 : 5) quantize_rows_ker
   uint8_t *q = a.q + row * a.ldq + (int64_t)block * SCALE_BLOCK;
   float *scale = a.scales + row * blocks + block;
   const int64_t q_step = step * a.ldq, scale_step = step * blocks;
-  Eight<T> e[2], next[2];
-  e[0].clear();
-  e[1].clear();
+  Eight<T> e[RUNS], next[RUNS];
+#pragma unroll
+  for (int i = 0; i < RUNS; ++i) e[i].clear();
   int from = source(row), from_next = source(row + step);
   fetch(from, e);
   const int64_t row0 = row - (unit >> lanes_log);   // the CTA's threads go round together
   for (int64_t r = row0; r < rows; r += step) {
     fetch(from_next, next);
     const int from_then = source(row + 2 * step);
-    float v[16];
-    e[0].values(v);
-    e[1].values(v + 8);
-    float amax = max_of<16>(v, 0.0f);
+    float amax = Eight<T>::largest(e, RUNS);
 #pragma unroll
-    for (int d = QR_LANES / 2; d; d >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, d));
+    for (int d = LANES / 2; d; d >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, d));
     if (__any_sync(0xffffffffu, !finite(amax))) {
-      amax = finite_max_of<16>(v, 0.0f);
+      amax = 0.0f;
 #pragma unroll
-      for (int d = QR_LANES / 2; d; d >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, d));
+      for (int i = 0; i < RUNS; ++i) {
+        float v[8];
+        e[i].values(v);
+        amax = finite_max_of<8>(v, amax);
+        e[i].nan_unless_finite();
+      }
 #pragma unroll
-      for (int j = 0; j < 16; ++j) v[j] = finite_or_nan(v[j]);
+      for (int d = LANES / 2; d; d >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, d));
     }
     if (from >= 0) {
       const int ex = scale_exponent(amax);
       const float inv = power_of_two(-ex);
-      if (WHOLE || (VEC && left == SCALE_BLOCK)) {
-        *reinterpret_cast<uint2 *>(q + t * 8) = make_uint2(pack4(v, inv), pack4(v + 4, inv));
-        *reinterpret_cast<uint2 *>(q + 64 + t * 8) = make_uint2(pack4(v + 8, inv), pack4(v + 12, inv));
-      } else {
 #pragma unroll
-        for (int j = 0; j < 16; ++j)
-          if (column(j) < left) q[column(j)] = (uint8_t)pack2(v[j] * inv, 0.0f);
+      for (int i = 0; i < RUNS; ++i) {
+        const uint2 w = e[i].packed(inv);
+        if (WHOLE || (VEC && left == SCALE_BLOCK)) {
+          *reinterpret_cast<uint2 *>(q + i * RUN + t * 8) = w;
+        } else {
+#pragma unroll
+          for (int j = 0; j < 8; ++j)
+            if (column(i * 8 + j) < left) q[column(i * 8 + j)] = (uint8_t)((j < 4 ? w.x : w.y) >> (8 * (j & 3)));
+        }
       }
       if (t == 0) *scale = power_of_two(ex);
     }
@@ -156,8 +209,8 @@ __global__ void __launch_bounds__(256, sizeof(T) == 4 ? 4 : 5) quantize_rows_ker
     row += step;
     from = from_next;
     from_next = from_then;
-    e[0] = next[0];
-    e[1] = next[1];
+#pragma unroll
+    for (int i = 0; i < RUNS; ++i) e[i] = next[i];
   }
 }
 
@@ -199,13 +252,7 @@ __global__ void __launch_bounds__(256) quantize_blocks_kernel(QuantArgs a, int64
             if (t * 8 + j < cols) w[j] = p[j];
         }
       }
-#pragma unroll
-      for (int k = 0; k < 8; ++k) {
-        float v[8];
-        e[k].values(v);
-        amax = max_of<8>(v, amax);
-      }
-      amax = cta_max(amax, part);
+      amax = cta_max(Eight<T>::largest(e, 8), part);
       const bool odd = !finite(amax);   // the same for all threads
       if (odd) {
         amax = 0.0f;
@@ -223,13 +270,8 @@ __global__ void __launch_bounds__(256) quantize_blocks_kernel(QuantArgs a, int64
 #pragma unroll
       for (int k = 0; k < 8; ++k) {
         if (row + 16 * k >= rows) break;
-        float v[8];
-        e[k].values(v);
-        if (odd) {
-#pragma unroll
-          for (int j = 0; j < 8; ++j) v[j] = finite_or_nan(v[j]);
-        }
-        const uint2 w = make_uint2(pack4(v, inv), pack4(v + 4, inv));
+        if (odd) e[k].nan_unless_finite();
+        const uint2 w = e[k].packed(inv);
         uint8_t *q = a.q + (r0 + row + 16 * k) * a.ldq + c0 + t * 8;
         if (t * 8 + 8 <= cols) {
           *reinterpret_cast<uint2 *>(q) = w;
@@ -262,9 +304,9 @@ template <typename T, bool VEC>
 cudaError_t launch_form(const QuantArgs &a, int num_sms, cudaStream_t s) {
   const int64_t blocks = scale_blocks(a.cols);
   if (a.block_rows == 1) {
-    int lanes_log = 5;
+    int lanes_log = sizeof(T) == 4 ? 5 : 6;
     while (lanes_log > 0 && blocks <= 1 << (lanes_log - 1)) --lanes_log;
-    const int64_t x = (blocks + (1 << lanes_log) - 1) >> lanes_log, rows = 256 / QR_LANES >> lanes_log;
+    const int64_t x = (blocks + (1 << lanes_log) - 1) >> lanes_log, rows = 256 / QR_LANES<T> >> lanes_log;
     // four rows a thread, and no more CTAs than eight for each SM
     int64_t y = (a.rows + 4 * rows - 1) / (4 * rows);
     y = y * x < num_sms * 8 ? (a.rows + rows - 1) / rows : y;

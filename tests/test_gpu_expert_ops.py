@@ -116,6 +116,25 @@ def test_quantize_edges_of_the_types(type):
         same_values(q, want)
 
 
+@pytest.mark.parametrize("type", [t for t in TYPES if TYPES[t] != torch.float32])
+def test_quantize_every_number_of_the_type(type):
+    """By magnitude (blocks of neighbours, the subnormal ones among them), mixed, and as signs alternate."""
+    every = torch.arange(1 << 16, dtype=torch.int32)
+    mixed = every[torch.randperm(1 << 16, generator=torch.Generator().manual_seed(1))]
+    signs = torch.stack([every[:1 << 15], every[1 << 15:]], 1)
+    x = torch.cat([every.view(-1, 1024), mixed.view(-1, 1024), signs.reshape(-1, 1024)]).to(torch.int16).cuda().view(TYPES[type])
+    for block_rows in (1, 128):
+        q = torch.zeros(x.shape, dtype=torch.uint8, device="cuda").view(torch.float8_e4m3fn)
+        scales = torch.zeros(-(-x.shape[0] // block_rows), 8, device="cuda")
+        assert ec.quantize(x, q, scales, block_rows) == 0
+        want, s = quantize64(x, block_rows)
+        assert np.array_equal(scales.double().cpu().numpy(), s)
+        same_values(q, want)
+        numbers = ~np.isnan(want)
+        assert np.array_equal((q.view(torch.uint8).cpu().numpy() >= 128)[numbers], (x < 0).cpu().numpy()[numbers] |
+                              ((x == 0) & (x.view(torch.int16) < 0)).cpu().numpy()[numbers])
+
+
 @pytest.mark.parametrize("cols", [64, 200, 1024])
 def test_quantize_gathers_rows(cols):
     gen = generator(cols)
