@@ -508,11 +508,31 @@ int shares_of_k(int64_t tiles, int64_t resident, int kblocks) {
   return s;
 }
 
+// Rows of a tile in the form of 256 rows: fewer where that comes to less time, for a group's last tile is cut off and a round of tiles
+// may be nearly empty.  A tile takes as long as what it loads, 128 weights and its rows.  How many tiles several groups have is an
+// estimate: fewer rows are taken when they are better by more than a few percent with two standard deviations more of tiles (of the
+// groups' last ones, each anything between none and all of a tile).  (us with 256 rows and this way: 5003 rows in 8 groups, N = 1000,
+// K = 1160 36.6 28.8; 16384 in 32, 1024, 2048 87 78; 1500 in one, 2048, 4096 29.0 27.4.)
+int tile_height(const ProductArgs &a, int tiles_n, int num_sms) {
+  const double live = (double)std::min(a.groups, a.rows);
+  auto time = [&](int high, double more) {
+    const double m = (double)a.rows / high;
+    return std::ceil((a.groups == 1 ? std::ceil(m) : std::max(m + 0.5 * live + more, live)) * tiles_n / num_sms) * (PT_ROWS + high);
+  };
+  int best = 256;
+  double least = (a.groups == 1 ? 1.0 : 0.94) * time(256, 0.0);
+  for (int high = 240; high >= 128; high -= 16) {
+    const double t = time(high, 0.58 * std::sqrt(live));
+    if (t < least) best = high, least = t;
+  }
+  return best;
+}
+
 // Rows of a tile: 32, 64, 128 (e4m3; with 16 bits two CTAs of 64 were as fast) with the rows on the N side, two CTAs of the first two
-// on an SM, or 256 (16-bit operands; e4m3: the wide form, 128 rows on the M side and 256 weights).  By the time that the tiles take in rounds of what is resident, from the
-// measured times of a k-step, in hundredths of a microsecond.  (us with 32, 64 and 256 rows in bf16, 32, 64, 128 and 256 in e4m3: 4096
-// rows, N = 1000, K = 4096 63 45 32 and 60 46 37 25; 300 rows 15 14 26 and 15 14 14 22; 2000 rows in eight groups 37 28 33 and 34 26 36 24;
-// 5000 in 32 89 74 66 and 76 64 60 48.)
+// on an SM, or up to 256 (16-bit operands; e4m3: the wide form, 128 rows on the M side and 256 weights).  By the time that the tiles take
+// in rounds of what is resident, from the measured times of a k-step, in hundredths of a microsecond.  (us with 32, 64 and 256 rows in
+// bf16, 32, 64, 128 and 256 in e4m3: 4096 rows, N = 1000, K = 4096 63 45 32 and 60 46 37 25; 300 rows 15 15 19 and 15 14 14 22; 2000 rows
+// in eight groups 37 29 31 and 34 26 36 24; 5000 in 32 89 74 66 and 76 64 60 48.)
 int choose_rows(const ProductArgs &a, bool scaled, bool gated, int kblocks, int num_sms) {
 #ifdef OCCAMY_TUNING
   if (const char *e = getenv("OCCAMY_PT_BN")) return atoi(e);
@@ -525,12 +545,14 @@ int choose_rows(const ProductArgs &a, bool scaled, bool gated, int kblocks, int 
   for (int i = 0; i < 4; ++i) {
     if (!scaled && i == 2) continue;
     const bool wide = scaled && i == 3;
-    const double m = wide ? 128 : rows_of[i], n = (wide ? 256 : PT_ROWS) / (gated ? 2 : 1);
+    const double n = (wide ? 256 : PT_ROWS) / (gated ? 2 : 1);
+    const int high = scaled || i < 3 ? rows_of[i] : tile_height(a, (int)std::ceil(a.N / n), num_sms);
+    const double m = wide ? 128 : high;
     const double tiles = std::max(a.groups == 1 ? std::ceil(a.rows / m) : a.rows / m + 0.5 * live, live) * std::ceil(a.N / n);
     const double slots = (double)num_sms * (i < 2 ? 2 : 1);
     const int shares = i < 3 ? shares_of_k((int64_t)tiles, (int64_t)slots, kblocks) : 1;
     const double full = tiles * shares / slots, rounds = std::max(1.0, 0.5 * (full + std::ceil(full)));
-    const double t = rounds * ((kblocks + shares - 1) / shares) * step[scaled][i] + (shares > 1 ? 300 : 0);
+    const double t = rounds * ((kblocks + shares - 1) / shares) * step[scaled][i] * (PT_ROWS + high) / (PT_ROWS + rows_of[i]) + (shares > 1 ? 300 : 0);
     if (i == 0 || t < least) best = i, least = t;
   }
   return rows_of[best];
@@ -624,8 +646,13 @@ cudaError_t launch_product(const ProductArgs &a, int num_sms, cudaStream_t s) {
 #ifdef OCCAMY_TC_TIMERS
   p.timers = tc_timer_words();
 #endif
-  const int tile_m = wide ? 128 : BN, tile_n = (wide ? 256 : PT_ROWS) / (gated ? 2 : 1);
+  const int tile_n = (wide ? 256 : PT_ROWS) / (gated ? 2 : 1);
   p.tiles_n = (int)((a.N + tile_n - 1) / tile_n);
+  p.height = BN == 256 ? tile_height(a, p.tiles_n, num_sms) : BN;
+#ifdef OCCAMY_TUNING
+  if (const char *e = getenv("OCCAMY_PT_HEIGHT")) p.height = std::min(atoi(e), BN);
+#endif
+  const int tile_m = wide ? 128 : p.height;
   // (rows of g groups fill at most so many tiles)
   const int64_t most_tiles =
       std::min<int64_t>((a.rows + std::min(a.groups, a.rows) * (tile_m - 1)) / tile_m * p.tiles_n, 1 << 28);

@@ -30,6 +30,7 @@ struct alignas(64) PtParams {
   int kblocks;                         // k-steps: blocks of 128 bytes along K
   int blocks_n;                        // scale blocks of a matrix along N
   int tiles_n, stages, splits, bufs;
+  int height;                          // rows of a tile, in the form of 256 up to so many
   uint32_t idesc;                      // instruction descriptor without N
   int vec_out;                         // 16-byte stores of the result are possible
   int *err;
@@ -207,7 +208,8 @@ __device__ __forceinline__ void pt_count_tiles(const PtParams &p, const PtGroups
     int begin = __shfl_up_sync(0xffffffffu, end, 1);
     if (lane == 0) begin = top;
     top = __shfl_sync(0xffffffffu, end, 31);
-    const int n = g < p.groups ? (end - begin + ROWS - 1) / ROWS : 0;
+    const int high = ROWS == 256 ? p.height : ROWS;
+    const int n = g < p.groups ? (end - begin + high - 1) / high : 0;
     int upto = n;
 #pragma unroll
     for (int d = 1; d < 32; d *= 2) {
@@ -236,10 +238,11 @@ __device__ __forceinline__ PtTile pt_decode(const PtParams &p, const PtGroups &t
   const int band = local / (PT_RASTER * p.tiles_n), in_band = local - band * PT_RASTER * p.tiles_n;
   const int height = min(PT_RASTER, all - band * PT_RASTER), n = in_band / height;
   const int m = band * PT_RASTER + in_band - n * height;
+  const int high = ROWS == 256 ? p.height : ROWS;
   PtTile tl;
   tl.g = lo;
-  tl.m0 = t.first[lo] + m * ROWS;
-  tl.rows = min(ROWS, t.last[lo] - tl.m0);
+  tl.m0 = t.first[lo] + m * high;
+  tl.rows = min(high, t.last[lo] - tl.m0);
   tl.n0 = n * WEIGHTS;
   return tl;
 }

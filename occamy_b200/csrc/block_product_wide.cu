@@ -5,9 +5,11 @@
 // operands, copies and scales together.  A thread holds 128 sums of its row.  For each k-step it waits for the TMEM buffer, reads
 // 16 columns at a time and adds them, scaled.  On an SM that is 256 cycles of fp32 arithmetic and 150 of TMEM reads against the 512
 // that the tensor core takes for the k-step, but all eight warps go through it together, from one TMEM buffer's barrier to the
-// next, and with what they wait on the way a k-step takes them 950: that is what bounds the kernel (8190 x 8192 x 4096: 275 us, 2.0
-// PFLOP/s; with the sums left out 253, with a quarter of the MMAs 279).  Tried: sixteen warps of 64 columns (310 us: no registers for
-// their loads), loads of 32 or 64 columns (spills), pairs of CTAs (cta_group::2, 289: the second CTA's sums come later still).
+// next, and with what they wait on the way a k-step takes them 950: that is what bounds the kernel (8190 x 8192 x 4096: 271 us, 2.0
+// PFLOP/s; without the sums 250, without the TMEM reads 254, without both 224, and of that the loads alone take 167, 19 TB/s out of L2).
+// Tried: sixteen warps of 64 columns (310: no registers for their loads), loads of 32 or 64 columns (spills), either half of the weights
+// committed by itself (291 against 280 then), pairs of CTAs (cta_group::2, 288 to 330: less to load, but the second CTA's sums hold up
+// both).
 #include <algorithm>
 #include <mutex>
 

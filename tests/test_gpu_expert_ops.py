@@ -404,6 +404,35 @@ def test_products_in_every_form(rows, type, act, out_type, bias, gathered):
         assert torch.equal(out, again)
 
 
+@pytest.mark.parametrize("sizes", [[5003, 0, 0, 0, 0, 0, 0, 0], [0, 700, 600, 650, 620, 1, 1200, 1232], [625] * 7 + [628],
+                                   [160, 320, 480, 640, 800, 960, 1120, 523], [161, 321, 481, 641, 801, 961, 1121, 516],
+                                   [1500], [1100], [2304]])
+@pytest.mark.parametrize("act,n,gathered", [("none", 1000, False), ("gated", 512, False), ("relu", 1096, True)])
+def test_heights_of_tiles(sizes, act, n, gathered):
+    """Tiles of up to 256 rows are lower where that saves a round; the groups are not what was reckoned with."""
+    k, groups, used = 328, len(sizes), sum(sizes)
+    both = (2,) if act == "gated" else ()
+    gen = generator(used + n)
+    sources = 900 if gathered else used
+    a = torch.randn(sources, k, generator=gen, device="cuda").half()
+    b = (torch.randn(groups, *both, n, k, generator=gen, device="cuda") * k ** -0.5).half()
+    index = torch.randint(-1, sources + 1, (used,), generator=gen, device="cuda", dtype=torch.int32) if gathered else None
+    offsets = torch.tensor(list(itertools.accumulate([0] + sizes)), dtype=torch.int32, device="cuda")
+    base, out = kept(used, n, torch.float32)
+    before = rt.form_counters()["product_256"]
+    assert ec.grouped(a, offsets, b, out, act=act, index=index) == 0
+    assert rt.form_counters()["product_256"] == before + 1 or used < 1500
+    av = a.double()
+    if gathered:
+        there = (index >= 0) & (index < sources)
+        av = torch.where(there[:, None], av[index.long().clamp(0, sources - 1)], torch.zeros_like(av[:1]))
+    for g in range(groups):
+        lo, hi = sum(sizes[:g]), sum(sizes[:g + 1])
+        if lo < hi:
+            ec.close(out[lo:hi], *ec.product64(av[lo:hi], b[g].double(), None, act, torch.float32))
+    assert (base[:, n:] == KEEP).all()
+
+
 def test_forms_of_one_group():
     """The counters say which tiles calls take."""
     gen = generator(1)
@@ -427,7 +456,7 @@ def test_forms_of_one_group():
     assert one("e4m3", 300, 4096, 2048) == ["product_128"]
     assert one("e4m3", 2048, 4096, 1024) == ["product_256"]
     assert one("fp16", 20, 4096, 2048) == ["product_32"]
-    assert one("fp16", 300, 4096, 2048) == ["product_64"]
+    assert one("fp16", 600, 1000, 4096) == ["product_64"]
     assert one("fp16", 4096, 4096, 256) == ["product_256"]
 
 
