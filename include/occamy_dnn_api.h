@@ -292,7 +292,8 @@ int occamy_quantize_e4m3(const void *x, int xType, int64_t xRows, int64_t cols, 
 /* out[M][N] = act(A B^T + bias) of e4m3 A[M][K] and B[N][K]: the value of A[m][k] is a * scaleA[m][k / 128], that of B[n][k]
  * b * scaleB[n / 128][k / 128]; both scale arrays are dense, of any fp32 numbers.  bias [N] or null, fp32.  activMode as in
  * DNNConvBiasActivFunc and DNNActiveFunc, 0 sigmoid, 1 ReLU, 2 tanh, 3 clip to [0, 6], 5 identity, and 6: x * sigmoid(x).
- * outType 0, 1 or 2.  A and B start at multiples of 16 bytes, and so do their rows (lda % 16 == 0, ldb % 16 == 0). */
+ * outType 0, 1 or 2.  A and B start at multiples of 16 bytes, and so do their rows (lda % 16 == 0, ldb % 16 == 0).  M and N (below:
+ * rows, and rows of all matrices of B) are at most 2^31 - 1024. */
 int occamy_matmul_e4m3(const void *a, int64_t lda, const float *scaleA, const void *b, int64_t ldb,
                        const float *scaleB, const float *bias, int64_t M, int64_t N, int64_t K,
                        int64_t activMode, void *out, int outType, int64_t ldo, cudaStream_t stream);

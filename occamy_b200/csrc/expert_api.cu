@@ -17,7 +17,7 @@ namespace {
 
 constexpr int MAX_DEVICES = 64;
 constexpr int NO_DEVICE = -1, TOO_SMALL = -2, BAD_ARGUMENT = -3, FAILED = -4, BAD_POINTER = -5, CAPTURED = -6;
-constexpr int64_t MOST_EXPERTS = 1024, MOST_CHOICES = 32;
+constexpr int64_t MOST_EXPERTS = 1024, MOST_CHOICES = 32, MOST_ROWS = (1ll << 31) - 1024;
 
 // Calls may come from several host threads; what they share (the tensor registry, counters, first-use set-up) is
 // not made for that.
@@ -161,7 +161,8 @@ int product(Call &call, ProductArgs &p, cudaStream_t stream) {
   const int both = p.act == ACT_GATED_SILU ? 2 : 1, es = elem_size(p.type);
   const int64_t mats = p.groups * both;
   if (!real_type(p.out_type)) return refuse(BAD_ARGUMENT, who, "type of the result");
-  if (mats * p.N > INT_MAX) return refuse(BAD_ARGUMENT, who, "more than 2^31 - 1 rows of weights");
+  // (the kernels' 32-bit row and weight numbers go up to a tile past the end)
+  if (p.rows > MOST_ROWS || mats * p.N > MOST_ROWS) return refuse(BAD_ARGUMENT, who, "more than 2^31 - 1024 rows of A or of weights");
   if (!row_length(p.lda, p.K, p.a_rows, es) || !row_length(p.ldb, p.K, mats * p.N, es) || !row_length(p.ldo, p.N, p.rows, 4))
     return refuse(BAD_ARGUMENT, who, "distance between rows out of range");
   if (p.lda * es % 16 || p.ldb * es % 16)

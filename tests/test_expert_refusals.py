@@ -88,6 +88,14 @@ def test_empty_problems_are_done(lib):
     assert call(lib.occamy_combine_experts, COMBINE, tokens=0) == 0
 
 
+@pytest.mark.parametrize("at", ["m", "n"])
+def test_products_refuse_what_32_bits_do_not_number(lib, at):
+    k = dict(ldo=2 ** 31) if at == "n" else {}
+    assert call(lib.occamy_matmul_e4m3, MATMUL, **{at: 2 ** 31 - 1023}, **k) == -3
+    grouped = dict(rows=2 ** 31 - 1023, a_rows=2 ** 31 - 1023) if at == "m" else dict(n=2 ** 31 // GROUPED["groups"], ldo=2 ** 31)
+    assert call(lib.occamy_matmul_grouped, GROUPED, **grouped) == -3
+
+
 def test_no_device_is_an_error(lib):
     """On a machine without a GPU the calls say so; they do not end the process."""
     import torch
