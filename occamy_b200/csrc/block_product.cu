@@ -91,13 +91,15 @@ __global__ void __launch_bounds__(PT_THREADS, BN <= 64 ? 2 : 1) block_product_ke
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
   }
   pdl_launch_dependents();
-  pdl_wait();
+  // (without offsets nothing here was written by the kernel before: this much of the start goes on beside its end)
+  if (p.offsets) pdl_wait();
   pt_read_groups<PT_THREADS>(p, groups);
   __syncthreads();
   if (warp == 0) pt_count_tiles<BN>(p, groups, lane);
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
+  if (!p.offsets) pdl_wait();
   const uint32_t tmem = *tmem_holder;
   const int splits = p.splits, rank = splits > 1 ? (int)cluster_ctarank() : 0;
   const int total = pt_total(p, groups);
@@ -156,7 +158,10 @@ __global__ void __launch_bounds__(PT_THREADS, BN <= 64 ? 2 : 1) block_product_ke
       const float x[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
 #pragma unroll
       for (int j = 0; j < 8; ++j) r[j] = x[j] + (bias && n_lane + j < n_tile ? bias[j] : 0.0f);
-      if (p.act != ACT_IDENTITY) {
+      if (p.act == ACT_RELU) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) r[j] = r[j] < 0.0f ? 0.0f : r[j];
+      } else if (p.act != ACT_IDENTITY) {
 #pragma unroll
         for (int j = 0; j < 8; ++j) r[j] = activate(r[j], p.act);
       }
@@ -327,6 +332,8 @@ __global__ void __launch_bounds__(PT_THREADS, BN <= 64 ? 2 : 1) block_product_ke
     uint32_t buf_phase = 0;
     for (int tile = tile0; tile < total && !err_code; tile += tstep) {
       const PtTile tl = decode(tile);
+      if (splits > 1 && p.bias && n_lane < p.N - tl.n0)   // there when the sums are
+        asm volatile("prefetch.global.L1 [%0];" ::"l"(p.bias + (int64_t)tl.g * SETS * p.N + tl.n0 + n_lane));
 #pragma unroll
       for (int i = 0; i < CW / 2; ++i) acc[i] = 0;
       for (int kb = k0; kb < k1; kb += PER) {
@@ -448,22 +455,19 @@ __global__ void __launch_bounds__(PT_THREADS, BN <= 64 ? 2 : 1) block_product_ke
 #pragma unroll 1
         for (int g = 0; g < NG && c0 + g * 8 < tl.rows; ++g) {
           if ((ew * NG + g) % splits != rank) continue;
-          // (four CTAs' sums on their way together: one after another took 2 us)
+          // (all CTAs' sums on their way together: one after another took 2 us)
           float t[8] = {};
           const uint32_t from = sW + (uint32_t)(g * 4 * EW * 32 + (int)threadIdx.x - 32 * PT_EPI_WARP) * 8u;
-          for (int r0 = 0; r0 < splits; r0 += 4) {
-            float2 x[4][4];
+          float2 x[8][4];
 #pragma unroll
-            for (int r = 0; r < 4; ++r)
+          for (int r = 0; r < 8; ++r)
 #pragma unroll
-              for (int j = 0; j < 4; ++j)
-                x[r][j] = r0 + r < splits ? ld_cluster_f32x2(cluster_map(from, (uint32_t)(r0 + r)) + j * (EW * 32 * 8))
-                                          : make_float2(0.0f, 0.0f);
+            for (int j = 0; j < 4; ++j)
+              x[r][j] = r < splits ? ld_cluster_f32x2(cluster_map(from, (uint32_t)r) + j * (EW * 32 * 8)) : make_float2(0.0f, 0.0f);
 #pragma unroll
-            for (int r = 0; r < 4; ++r)
+          for (int r = 0; r < 8; ++r)
 #pragma unroll
-              for (int j = 0; j < 4; ++j) t[2 * j] += x[r][j].x, t[2 * j + 1] += x[r][j].y;
-          }
+            for (int j = 0; j < 4; ++j) t[2 * j] += x[r][j].x, t[2 * j + 1] += x[r][j].y;
           finish(tl, g, [&](int, auto &&put) {
 #pragma unroll
             for (int j = 0; j < 4; ++j) put(j, t[2 * j], t[2 * j + 1]);
