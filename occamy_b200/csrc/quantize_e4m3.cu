@@ -125,7 +125,7 @@ struct Eight {
 // keeps its place in the row and goes from row to row, the next one's elements on their way while it works on these.
 // WHOLE: VEC and no block is cut off.  What bounds it is the first-level cache (77 %: lines come in halves) and instructions (61 % of the
 // issue slots): 16384 gathered rows of 4096 bf16 27 us, eight threads a block with all arithmetic in 32 bits 31, without the next
-// row on its way and two CTAs more on an SM 29.
+// row on its way and two CTAs more on an SM 29, eight threads for two blocks (lines read whole, more registers) 31.
 template <typename T>
 constexpr int QR_LANES = sizeof(T) == 4 ? 8 : 4;
 template <typename T, bool VEC, bool WHOLE>
