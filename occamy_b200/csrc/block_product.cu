@@ -89,8 +89,9 @@ __global__ void __launch_bounds__(PT_THREADS, BN <= 64 ? 2 : 1) block_product_ke
                  "r"(COLS)
                  : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    // (not before: a CTA of the next kernel that took the columns first would keep them until this one ends)
+    pdl_launch_dependents();
   }
-  pdl_launch_dependents();
   // (without offsets nothing here was written by the kernel before: this much of the start goes on beside its end)
   if (p.offsets) pdl_wait();
   pt_read_groups<PT_THREADS>(p, groups);

@@ -80,8 +80,9 @@ __global__ void __launch_bounds__(PT_THREADS, 1) block_product_wide_kernel(const
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_u32((const void *)tmem_holder))
                  : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    // (not before: a CTA of the next kernel that took the columns first would keep them until this one ends)
+    pdl_launch_dependents();
   }
-  pdl_launch_dependents();
   pdl_wait();
   pt_read_groups<PT_THREADS>(p, groups);
   __syncthreads();
