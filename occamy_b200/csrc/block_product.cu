@@ -67,12 +67,13 @@ __global__ void __launch_bounds__(PT_THREADS, BN <= 64 ? 2 : 1) block_product_ke
   const PtGroups groups = {words + 4, words + 4 + p.groups, words + 4 + 2 * p.groups};
 
   const int warp = warp_index(), lane = threadIdx.x & 31;
+  const bool indexed = BN < 256 && p.index;   // (choose_rows)
   constexpr uint32_t COLS = BN >= 128 ? 512 : BN * 4;
   if (threadIdx.x == 0) {
-    if (!p.index) tma_prefetch_map(&p.ta);
+    if (!indexed) tma_prefetch_map(&p.ta);
     tma_prefetch_map(&p.tb);
     for (int s = 0; s < stages; ++s) {
-      mbar_init(full_bar(s), p.index ? 1 + 32 * PT_GATHERERS : 1);   // loads, lanes that copy rows chosen by an index
+      mbar_init(full_bar(s), indexed ? 1 + 32 * PT_GATHERERS : 1);   // loads, lanes that copy rows chosen by an index
       mbar_init(empty_bar(s), 1);
     }
     for (int b = 0; b < bufs; ++b) {
@@ -171,11 +172,12 @@ __global__ void __launch_bounds__(PT_THREADS, BN <= 64 ? 2 : 1) block_product_ke
                  n_tile - n_lane);
   };
 
-  // The sums' warps take the registers that the others do without: (256 x 48 + 256 x 208) = 512 x 128, of two CTAs (256 x 40 + 256 x
-  // 88) = 512 x 64.  (Each at the head of its roles: behind a point where both come together the compiler keeps to the smaller
-  // number.)
+  // The sums' warps take the registers that the others do without: (256 x 48 + 256 x 208) = 512 x 128 (256 rows: 56 and 200, with
+  // which nothing is spilled), of two CTAs (256 x 40 + 256 x 88) = 512 x 64.  (Each at the head of its roles: behind a point where both
+  // come together the compiler keeps to the smaller number.)
   if (warp < PT_EPI_WARP) {
   if constexpr (BN <= 64) asm volatile("setmaxnreg.dec.sync.aligned.u32 40;");
+  else if constexpr (BN == 256) asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
   else asm volatile("setmaxnreg.dec.sync.aligned.u32 48;");
   if (warp == 0) {
     // ------------------------------------------------------------ loads
@@ -184,7 +186,7 @@ __global__ void __launch_bounds__(PT_THREADS, BN <= 64 ? 2 : 1) block_product_ke
     uint32_t phase = 0;
     for (int tile = tile0; tile < total && !err_code; tile += tstep) {
       const PtTile tl = decode(tile);
-      const int boxes = p.index ? 0 : (tl.rows + PT_BOX - 1) / PT_BOX;
+      const int boxes = indexed ? 0 : (tl.rows + PT_BOX - 1) / PT_BOX;
       const uint32_t bytes = W_BYTES + (uint32_t)boxes * (PT_BOX * 128u);
       for (int kb = k0; kb < k1; ++kb) {
         if (!TCT_WAIT(0, mbar_wait_warp(empty_bar(stage), phase ^ 1u, abort_flag))) {
@@ -232,7 +234,7 @@ __global__ void __launch_bounds__(PT_THREADS, BN <= 64 ? 2 : 1) block_product_ke
           err_code = 3;
           break;
         }
-        if (p.index) fence_async_smem();
+        if (indexed) fence_async_smem();
         tc_fence_after();
         const uint32_t d = tmem + (uint32_t)(buf * BN);
         const uint32_t a = w_lo + (uint32_t)stage * (W_BYTES >> 4), b = r_lo + (uint32_t)stage * (R_BYTES >> 4);
@@ -257,9 +259,11 @@ __global__ void __launch_bounds__(PT_THREADS, BN <= 64 ? 2 : 1) block_product_ke
     TCT_FLUSH(1)
   } else if (warp >= PT_GATHER_WARP) {
     // ------------------------------------------------------------ rows chosen by an index
-    if (p.index)
-      err_code = pt_gather_role<BN, PT_GATHERERS>(p, tile0, total, tstep, k0, k1, sR, stages, warp - PT_GATHER_WARP, lane, abort_flag,
-                                                  decode, full_bar, empty_bar);
+    if constexpr (BN < 256) {
+      if (p.index)
+        err_code = pt_gather_role<BN, PT_GATHERERS>(p, tile0, total, tstep, k0, k1, sR, stages, warp - PT_GATHER_WARP, lane, abort_flag,
+                                                    decode, full_bar, empty_bar);
+    }
   } else {
     // ------------------------------------------------------------ scales
     // sA * sB of every column, one k-step after another.
@@ -326,6 +330,7 @@ __global__ void __launch_bounds__(PT_THREADS, BN <= 64 ? 2 : 1) block_product_ke
   } else {
     // ------------------------------------------------------------ sums and results
     if constexpr (BN <= 64) asm volatile("setmaxnreg.inc.sync.aligned.u32 88;");
+    else if constexpr (BN == 256) asm volatile("setmaxnreg.inc.sync.aligned.u32 200;");
     else asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
     TCT_DECL
     uint64_t acc[CW / 2];                  // sums of weight `lane` of the quadrant and columns c0 + 2 i, 2 i + 1
@@ -537,18 +542,21 @@ int tile_height(const ProductArgs &a, int tiles_n, int num_sms) {
 // on an SM, or up to 256 (16-bit operands; e4m3: the wide form, 128 rows on the M side and 256 weights).  By the time that the tiles take
 // in rounds of what is resident, from the measured times of a k-step, in hundredths of a microsecond.  (us with 32, 64 and 256 rows in
 // bf16, 32, 64, 128 and 256 in e4m3: 4096 rows, N = 1000, K = 4096 63 45 32 and 60 46 37 25; 300 rows 15 15 19 and 15 14 14 22; 2000 rows
-// in eight groups 37 29 31 and 34 26 36 24; 5000 in 32 89 74 66 and 76 64 60 48.)
+// in eight groups 37 29 31 and 34 26 36 24; 5000 in 32 89 74 66 and 76 64 60 48.)  Rows chosen by an index are copied at 18 bytes a
+// cycle of an SM, whatever the form: 16-bit tiles of 256 rows would wait for them and do without an index (16384 rows in 32 groups, gated,
+// 1024 x 2048 bf16: 32, 64 and 256 rows 259 199 264; without an index 266 172 144).
 int choose_rows(const ProductArgs &a, bool scaled, bool gated, int kblocks, int num_sms) {
 #ifdef OCCAMY_TUNING
-  if (const char *e = getenv("OCCAMY_PT_BN")) return atoi(e);
+  if (const char *e = getenv("OCCAMY_PT_BN")) return !scaled && a.index ? std::min(atoi(e), 64) : atoi(e);
 #endif
   static const int rows_of[4] = {32, 64, 128, 256};
-  static const int step[2][4] = {{24, 32, 0, 40}, {43, 63, 50, 56}};
+  static const int steps[3][4] = {{24, 32, 0, 40}, {43, 63, 50, 56}, {28, 42, 0, 0}};
+  const int *step = steps[scaled ? 1 : a.index ? 2 : 0];
   const double live = (double)std::min(a.groups, a.rows);
   int best = 0;
   double least = 0;
   for (int i = 0; i < 4; ++i) {
-    if (!scaled && i == 2) continue;
+    if (!step[i]) continue;
     const bool wide = scaled && i == 3;
     const double n = (wide ? 256 : PT_ROWS) / (gated ? 2 : 1);
     const int high = scaled || i < 3 ? rows_of[i] : tile_height(a, (int)std::ceil(a.N / n), num_sms);
@@ -557,7 +565,7 @@ int choose_rows(const ProductArgs &a, bool scaled, bool gated, int kblocks, int 
     const double slots = (double)num_sms * (i < 2 ? 2 : 1);
     const int shares = i < 3 ? shares_of_k((int64_t)tiles, (int64_t)slots, kblocks) : 1;
     const double full = tiles * shares / slots, rounds = std::max(1.0, 0.5 * (full + std::ceil(full)));
-    const double t = rounds * ((kblocks + shares - 1) / shares) * step[scaled][i] * (PT_ROWS + high) / (PT_ROWS + rows_of[i]) + (shares > 1 ? 300 : 0);
+    const double t = rounds * ((kblocks + shares - 1) / shares) * step[i] * (PT_ROWS + high) / (PT_ROWS + rows_of[i]) + (shares > 1 ? 300 : 0);
     if (i == 0 || t < least) best = i, least = t;
   }
   return rows_of[best];
