@@ -1916,6 +1916,11 @@ bool occ::entry_takes_pool(const Entry &e) {
 // ---------------------------------------------------------------- made again
 void occ::flush_held_back() { flush_pending(); }
 bool occ::anything_held_back() { return g_pending.active; }
+bool occ::in_live_pool(const void *p) {
+  for (const PoolRec &r : g_pools)
+    if ((uintptr_t)p >= (uintptr_t)r.base && (uintptr_t)p < (uintptr_t)r.base + r.bytes) return true;
+  return false;
+}
 
 // The call of entry `e`, its pointers where `place` says; `host` is the source of a constant.
 void occ::run_again(const Entry &e, const std::function<void *(void *)> &place, const void *host) {

@@ -36,8 +36,9 @@ int refuse(int code, const char *who, const char *why, ...) {
 // One call: the current device, the pointers it was given, and the runtime's own stream.
 //
 // Memory that the runtime knows (wrapDNNMalloc, a pool) may not hold yet what it stands for: a zero fill or an upload that
-// is put off, a result kept in another format, a convolution held back.  Such tensors are brought up to date first, on the
-// runtime's stream; the caller's stream waits for that, and the runtime's for the call.
+// is put off, a result kept in another format, a convolution held back, a recorded inference whose calls wait for their graph.
+// Such tensors are brought up to date first, on the runtime's stream; the caller's stream waits for that, and the runtime's for
+// the call.
 class Call {
  public:
   Call(const char *who, cudaStream_t stream) : who_(who), stream_(stream) {}
@@ -100,7 +101,8 @@ class Call {
     }
     if (at.type != cudaMemoryTypeManaged && (at.type != cudaMemoryTypeDevice || at.device != device_))
       return refuse(BAD_POINTER, who_, "an address is not memory of the current device");
-    if (!reg_find(p)) return 0;
+    // (a tensor of an inference that is being replayed is not on record until its calls are made one by one)
+    if (!reg_find(p) && !in_live_pool(p)) return 0;
     if (stream_ != rt().stream && capturing())
       return refuse(CAPTURED, who_, "memory of the runtime's own cannot be used while the stream is captured");
     if (!settled_) {

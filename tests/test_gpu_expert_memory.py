@@ -1,0 +1,114 @@
+"""The 8-bit and grouped operators on memory that the runtime hands out: what such memory stands for may not be there yet,
+and later calls of the runtime have to see what was written."""
+import numpy as np
+import pytest
+import torch
+
+import expert_calls as ec
+from calls import Inference, rand
+from helpers import max_rel_err
+from occamy_b200 import runtime as rt
+from oracle import ref
+from test_gpu_expert_ops import quantize64, same_values
+
+pytestmark = pytest.mark.gpu
+
+PASSES = 10   # recorded, fused, quiet, captured once per pool block, then replayed
+SHAPE = (1, 16, 12, 12)
+
+
+@pytest.fixture(autouse=True)
+def no_errors(native_libs):
+    rt.set_math_mode(rt.MATH_F16)   # (twenty layers: bf16 storage alone would be off by 5e-2)
+    rt.lib().occamy_set_cross_call_fusion(0)   # forgets what was recorded: programs that begin alike are not replayed
+    rt.lib().occamy_set_cross_call_fusion(1)
+    rt.last_error(clear=True)
+    yield
+    rt.synchronize()
+    rt.set_math_mode(rt.MATH_BF16)
+    assert rt.last_error(clear=True) == 0
+
+
+def quantize(x, rows, cols, stream):
+    """fp32 rows at address x; (q, scales) as torch tensors."""
+    q = torch.zeros(rows, cols, dtype=torch.uint8, device="cuda").view(torch.float8_e4m3fn)
+    scales = torch.zeros(rows, ec.blocks(cols), device="cuda")
+    torch.cuda.synchronize()
+    assert rt.lib().occamy_quantize_e4m3(x, rt.F32, rows, cols, cols, None, rows, 1, q.data_ptr(), cols, scales.data_ptr(),
+                                         stream.cuda_stream) == 0
+    return q, scales
+
+
+def same_quantised(got, x):
+    torch.cuda.synchronize()
+    want, scales = quantize64(torch.from_numpy(x), 1)
+    assert np.array_equal(got[1].double().cpu().numpy(), scales)
+    same_values(got[0], want)
+
+
+def copy_rows(src, dst, stream):
+    """A torch tensor's rows to the fp32 rows at address dst, as a weighted sum of one row each."""
+    rows, cols = src.shape
+    position = torch.arange(rows, dtype=torch.int32, device="cuda")
+    ones = torch.ones(rows, device="cuda")
+    torch.cuda.synchronize()
+    assert rt.lib().occamy_combine_experts(src.data_ptr(), rt.F32, rows, cols, position.data_ptr(), ones.data_ptr(), rows, 1,
+                                           cols, dst, rt.F32, cols, stream.cuda_stream) == 0
+    return position, ones
+
+
+class Layers:
+    """Twenty convolutions of a fresh input; after layer `at` something else may happen to its result."""
+
+    def __init__(self):
+        self.w = [rand(i, 16, 16, 3, 3, scale=0.1) for i in range(20)]
+        self.b = [rand(100 + i, 16) for i in range(20)]
+
+    def run(self, x, at=None, then=None):
+        with Inference() as f:
+            y = f.put(x)
+            for i, (w, b) in enumerate(zip(self.w, self.b)):
+                y, _ = f.conv(y, SHAPE, f.put(w), w.shape, f.put(b), (1, 1), act=1)
+                if i == at:
+                    y = then(f, y) or y
+            return f.get(y, SHAPE)
+
+    def want(self, x, first=0):
+        for w, b in zip(self.w[first:], self.b[first:]):
+            x = ref.conv2d(x, w, b, (1, 1), act=1)
+        return x
+
+
+@pytest.mark.parametrize("at", [2, 14, 19])
+def test_results_of_a_replayed_inference(at):
+    """In the middle of an inference whose calls so far wait for a graph to be launched in their place, a call on another stream
+    reads one of their results."""
+    model, stream = Layers(), torch.cuda.Stream()
+    for i in range(PASSES):
+        x = rand(200 + i, *SHAPE)
+        assert max_rel_err(model.run(x), model.want(x)) <= 2e-2
+    seen = {}
+
+    def then(f, y):
+        seen["q"] = quantize(y, 16, 144, stream)
+        seen["y"] = f.get(y, SHAPE)
+    x = rand(300, *SHAPE)
+    got = model.run(x, at, then)
+    same_quantised(seen["q"], seen["y"].reshape(16, 144))
+    assert max_rel_err(got, model.want(x)) <= 2e-2
+
+
+@pytest.mark.parametrize("at", [2, 14])
+def test_writes_in_a_replayed_inference(at):
+    """The same, and what the call writes is the next layer's input."""
+    model, stream = Layers(), torch.cuda.Stream()
+    for i in range(PASSES):
+        model.run(rand(200 + i, *SHAPE))
+    z = rand(301, *SHAPE)
+    src = torch.from_numpy(z.reshape(16, 144)).cuda()
+    kept = []
+
+    def then(f, y):
+        kept.append(copy_rows(src, y, stream))
+    got = model.run(rand(300, *SHAPE), at, then)
+    assert max_rel_err(got, model.want(z, at + 1)) <= 2e-2
