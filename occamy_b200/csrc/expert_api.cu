@@ -3,6 +3,7 @@
 #include <climits>
 #include <cstdarg>
 #include <mutex>
+#include <vector>
 
 #include "expert_ops.h"
 #include "graph_replay.h"
@@ -68,14 +69,27 @@ class Call {
     }
     return 0;
   }
-  // Device memory that the call reads / writes; null is passed over.  `align`: of the address, in bytes.
-  int in(const void *p, size_t align) { return use(p, align, false); }
-  int out(void *p, size_t align) { return use(p, align, true); }
+  // `bytes` of device memory that the call reads / writes; null is passed over.  `align`: of the address, in bytes.
+  int in(const void *p, int64_t bytes, size_t align) { return use(p, bytes, align, false); }
+  int out(void *p, int64_t bytes, size_t align) { return use(p, bytes, align, true); }
 
-  // Before the launches.  Nothing has been enqueued on the caller's stream so far.
+  // When all memory is known and nothing can be refused any more but a capture, before the launches: nothing has been enqueued so far.
   int begin() {
-    if (!tracked_ || stream_ == rt().stream) return 0;
-    return order(rt().stream, stream_);
+    bool tracked = false;
+    // (a tensor of an inference that is being replayed is not on record until its calls are made one by one)
+    for (int i = 0; i < count_ && !tracked; ++i) tracked = in_live_pool(uses_[i].p) || !records(uses_[i]).empty();
+    if (!tracked) return 0;
+    if (stream_ != rt().stream && capturing())
+      return refuse(CAPTURED, who_, "memory of the runtime's own cannot be used while the stream is captured");
+    if (!settled_) occamy_internal_opaque_call();
+    tracked_ = true;
+    // A result may leave parts of its memory as they were: they have to be there too.  (An operand may be several tensors.)
+    for (int i = 0; i < count_; ++i)
+      for (uintptr_t t : records(uses_[i])) ensure_f32((const void *)t);
+    for (int i = 0; i < count_; ++i)
+      if (uses_[i].written)
+        for (uintptr_t t : records(uses_[i])) mark_f32((void *)t);
+    return stream_ == rt().stream ? 0 : order(rt().stream, stream_);
   }
   // `e`: of the launches.
   int end(cudaError_t e) {
@@ -91,7 +105,13 @@ class Call {
   const char *who() const { return who_; }
 
  private:
-  int use(const void *p, size_t align, bool written) {
+  struct Use {
+    const void *p;
+    int64_t bytes;
+    bool written;
+  };
+  static std::vector<uintptr_t> records(const Use &u) { return reg_within(u.p, (size_t)u.bytes); }
+  int use(const void *p, int64_t bytes, size_t align, bool written) {
     if (!p) return 0;
     if ((uintptr_t)p % align) return refuse(BAD_ARGUMENT, who_, "an address is not a multiple of %zu bytes", align);
     cudaPointerAttributes at;
@@ -101,17 +121,7 @@ class Call {
     }
     if (at.type != cudaMemoryTypeManaged && (at.type != cudaMemoryTypeDevice || at.device != device_))
       return refuse(BAD_POINTER, who_, "an address is not memory of the current device");
-    // (a tensor of an inference that is being replayed is not on record until its calls are made one by one)
-    if (!reg_find(p) && !in_live_pool(p)) return 0;
-    if (stream_ != rt().stream && capturing())
-      return refuse(CAPTURED, who_, "memory of the runtime's own cannot be used while the stream is captured");
-    if (!settled_) {
-      occamy_internal_opaque_call();
-      settled_ = true;
-    }
-    tracked_ = true;
-    ensure_f32(p);   // a result may leave parts of its memory as they were: they have to be there too
-    if (written) mark_f32(const_cast<void *>(p));
+    uses_[count_++] = {p, bytes, written};
     return 0;
   }
   bool capturing() const {
@@ -137,6 +147,8 @@ class Call {
   cudaStream_t stream_;
   int device_ = -1, num_sms_ = 0;
   bool settled_ = false, tracked_ = false;
+  Use uses_[8];
+  int count_ = 0;
 };
 
 bool extent(int64_t v) { return v >= 0 && v <= INT_MAX; }
@@ -145,6 +157,8 @@ bool real_type(int t) { return t == ELEM_F32 || t == ELEM_BF16 || t == ELEM_F16;
 bool row_length(int64_t ld, int64_t cols, int64_t rows, int size) {
   return ld >= cols && ld <= INT64_MAX / 16 && ld * size < (1ll << 40) && (rows <= 1 || ld <= INT64_MAX / 16 / rows);
 }
+// From the first element of such rows to the last, in bytes.
+int64_t span(int64_t rows, int64_t ld, int64_t cols, int size) { return rows ? ((rows - 1) * ld + cols) * size : 0; }
 bool linear_act(int64_t mode) {
   return mode == ACT_SIGMOID || mode == ACT_RELU || mode == ACT_TANH || mode == ACT_CLIP || mode == ACT_IDENTITY ||
          mode == ACT_SILU;
@@ -179,14 +193,15 @@ int product(Call &call, ProductArgs &p, cudaStream_t stream) {
     return refuse(BAD_ARGUMENT, who, "null pointer");
   if (!scaled) p.scale_a = p.scale_b = nullptr;
   TRY(call.open());
-  TRY(call.in(p.a, 16));
-  TRY(call.in(p.b, 16));
-  TRY(call.in(p.scale_a, 4));
-  TRY(call.in(p.scale_b, 4));
-  TRY(call.in(p.bias, 4));
-  TRY(call.in(p.index, 4));
-  TRY(call.in(p.offsets, 4));
-  TRY(call.out(p.out, elem_size(p.out_type)));
+  const int64_t blocks_k = scale_blocks(p.K);
+  TRY(call.in(p.a, span(p.a_rows, p.lda, p.K, es), 16));
+  TRY(call.in(p.b, span(mats * p.N, p.ldb, p.K, es), 16));
+  TRY(call.in(p.scale_a, p.a_rows * blocks_k * 4, 4));
+  TRY(call.in(p.scale_b, mats * scale_blocks(p.N) * blocks_k * 4, 4));
+  TRY(call.in(p.bias, mats * p.N * 4, 4));
+  TRY(call.in(p.index, p.rows * 4, 4));
+  TRY(call.in(p.offsets, (p.groups + 1) * 4, 4));
+  TRY(call.out(p.out, span(p.rows, p.ldo, p.N, elem_size(p.out_type)), elem_size(p.out_type)));
   p.err = rt().dev_err;
   TRY(call.begin());
   return call.end(launch_product(p, call.num_sms(), stream));
@@ -210,10 +225,10 @@ int occamy_quantize_e4m3(const void *x, int xType, int64_t xRows, int64_t cols, 
   if (rows == 0 || cols == 0 || xRows == 0) return 0;
   if (!x || !q || !scales) return refuse(BAD_ARGUMENT, call.who(), "null pointer");
   TRY(call.open());
-  TRY(call.in(x, elem_size(xType)));
-  TRY(call.in(index, 4));
-  TRY(call.out(q, 1));
-  TRY(call.out(scales, 4));
+  TRY(call.in(x, span(xRows, ldx, cols, elem_size(xType)), elem_size(xType)));
+  TRY(call.in(index, rows * 4, 4));
+  TRY(call.out(q, span(rows, ldq, cols, 1), 1));
+  TRY(call.out(scales, (rows + blockRows - 1) / blockRows * scale_blocks(cols) * 4, 4));
   TRY(call.begin());
   QuantArgs a = {x, xType, xRows, cols, ldx, index, rows, (int)blockRows, (uint8_t *)q, ldq, scales};
   return call.end(launch_quantize_e4m3(a, call.num_sms(), stream));
@@ -287,17 +302,17 @@ int occamy_route_experts(const void *logits, int type, int64_t tokens, int64_t e
   if (need && (!workspace || workspaceBytes < (int64_t)need))
     return refuse(TOO_SMALL, call.who(), "the workspace has to have %zu bytes", need);
   TRY(call.open());
-  TRY(call.out(offsets, 4));
+  TRY(call.out(offsets, (experts + 1) * 4, 4));
   if (tokens == 0) {
     TRY(call.begin());
     return call.end(cudaMemsetAsync(offsets, 0, (size_t)(experts + 1) * 4, stream));
   }
-  TRY(call.in(logits, elem_size(type)));
-  TRY(call.out(chosen, 4));
-  TRY(call.out(weights, 4));
-  TRY(call.out(order, 4));
-  TRY(call.out(position, 4));
-  TRY(call.out(workspace, 4));
+  TRY(call.in(logits, span(tokens, ldl, experts, elem_size(type)), elem_size(type)));
+  TRY(call.out(chosen, tokens * k * 4, 4));
+  TRY(call.out(weights, tokens * k * 4, 4));
+  TRY(call.out(order, tokens * k * 4, 4));
+  TRY(call.out(position, tokens * k * 4, 4));
+  TRY(call.out(workspace, (int64_t)need, 4));
   TRY(call.begin());
   RouteArgs a = {logits, type, tokens, experts, ldl, (int)k, normalise != 0, chosen, weights, offsets, order, position,
                  (int32_t *)workspace};
@@ -319,10 +334,10 @@ int occamy_combine_experts(const void *y, int type, int64_t yRows, int64_t ldy, 
   if (tokens == 0 || N == 0) return 0;
   if ((yRows && !y) || !position || !weights || !out) return refuse(BAD_ARGUMENT, call.who(), "null pointer");
   TRY(call.open());
-  if (yRows) TRY(call.in(y, elem_size(type)));
-  TRY(call.in(position, 4));
-  TRY(call.in(weights, 4));
-  TRY(call.out(out, elem_size(outType)));
+  if (yRows) TRY(call.in(y, span(yRows, ldy, N, elem_size(type)), elem_size(type)));
+  TRY(call.in(position, tokens * k * 4, 4));
+  TRY(call.in(weights, tokens * k * 4, 4));
+  TRY(call.out(out, span(tokens, ldo, N, elem_size(outType)), elem_size(outType)));
   TRY(call.begin());
   CombineArgs a = {y, type, yRows, ldy, position, weights, tokens, k, N, out, outType, ldo};
   return call.end(launch_combine(a, call.num_sms(), stream));

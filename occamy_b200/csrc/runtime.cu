@@ -102,6 +102,16 @@ TensorRec *reg_find(const void *p, uintptr_t *base) {
   return &it->second;
 }
 
+std::vector<uintptr_t> reg_within(const void *p, size_t bytes) {
+  const auto &recs = rt().recs;
+  const uintptr_t lo = (uintptr_t)p, hi = lo + bytes;
+  std::vector<uintptr_t> found;
+  auto it = recs.upper_bound(lo);
+  if (it != recs.begin() && std::prev(it)->first + std::prev(it)->second.bytes > lo) --it;
+  for (; it != recs.end() && it->first < hi; ++it) found.push_back(it->first);
+  return found;
+}
+
 bool mode_f16() { return rt().mode == MATH_F16; }
 
 static bool is_in_format(const void *p, Fmt want, int64_t n, int64_t c, int64_t h, int64_t w) {

@@ -165,6 +165,8 @@ void reg_new(void *p, size_t bytes, Fmt fmt);
 void reg_drop_range(void *p, size_t bytes);
 // Record that contains p, or nullptr.  *base receives its base pointer.
 TensorRec *reg_find(const void *p, uintptr_t *base = nullptr);
+// Base pointers of the records that overlap [p, p+bytes).
+std::vector<uintptr_t> reg_within(const void *p, size_t bytes);
 // Whether p is memory of a pool that has not been given back (abi.cu).
 bool in_live_pool(const void *p);
 // Make the bytes behind p plain fp32 NCHW (memset, upload or layout conversion as needed).

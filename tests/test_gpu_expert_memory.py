@@ -112,3 +112,45 @@ def test_writes_in_a_replayed_inference(at):
         kept.append(copy_rows(src, y, stream))
     got = model.run(rand(300, *SHAPE), at, then)
     assert max_rel_err(got, model.want(z, at + 1)) <= 2e-2
+
+
+def test_operands_that_span_several_tensors():
+    """Neighbours in a pool, read as the rows of one matrix: one uploaded, one a convolution's result in the runtime's own format,
+    one that was never written."""
+    w, b = rand(1, 16, 16, 3, 3, scale=0.1), rand(2, 16)
+    stream = torch.cuda.Stream()
+    for i in range(4):
+        x = rand(400 + i, *SHAPE)
+        with Inference() as f:
+            px, pw, pb = f.put(x), f.put(w), f.put(b)
+            first = f.put(x)
+            assert first % 16 == 0
+            y, _ = f.conv(px, SHAPE, pw, w.shape, pb, (1, 1), act=1)
+            zero = f.place(x.nbytes)
+            assert (y - first, zero - y) == (x.nbytes, x.nbytes)
+            got = quantize(first, 48, 144, stream)
+            rows = np.concatenate([x.reshape(16, 144), f.get(y, SHAPE).reshape(16, 144), np.zeros((16, 144), np.float32)])
+            # the next inference finds something else where nothing is written here
+            f.put(x, at=zero - f.pool.value)
+        same_quantised(got, rows)
+
+
+def test_results_that_span_several_tensors():
+    """The same neighbours, written in one call: none of them stands for what it was before."""
+    w, b = rand(1, 16, 16, 3, 3, scale=0.1), rand(2, 16)
+    z = rand(3, 3, *SHAPE)
+    src = torch.from_numpy(z.reshape(48, 144)).cuda()
+    stream = torch.cuda.Stream()
+    for i in range(4):
+        x = rand(400 + i, *SHAPE)
+        with Inference() as f:
+            px, pw, pb = f.put(x), f.put(w), f.put(b)
+            first = f.put(x)
+            y, _ = f.conv(px, SHAPE, pw, w.shape, pb, (1, 1), act=1)
+            zero = f.place(x.nbytes)
+            kept = copy_rows(src, first, stream)
+            for p, part in zip((first, y, zero), z):
+                assert np.array_equal(f.get(p, SHAPE), part)
+            r = f.relu(y, SHAPE)
+            assert np.array_equal(f.get(r, SHAPE), np.maximum(z[1], 0))
+        del kept
