@@ -70,8 +70,9 @@ class Call {
     return 0;
   }
   // `bytes` of device memory that the call reads / writes; null is passed over.  `align`: of the address, in bytes.
-  int in(const void *p, int64_t bytes, size_t align) { return use(p, bytes, align, false); }
-  int out(void *p, int64_t bytes, size_t align) { return use(p, bytes, align, true); }
+  // `whole`: a result without gaps between its rows.
+  int in(const void *p, int64_t bytes, size_t align) { return use(p, bytes, align, false, false); }
+  int out(void *p, int64_t bytes, size_t align, bool whole = true) { return use(p, bytes, align, true, whole); }
 
   // When all memory is known and nothing can be refused any more but a capture, before the launches: nothing has been enqueued so far.
   int begin() {
@@ -84,8 +85,10 @@ class Call {
     if (!settled_) occamy_internal_opaque_call();
     tracked_ = true;
     // A result may leave parts of its memory as they were: they have to be there too.  (An operand may be several tensors.)
+    // One that fusion left unwritten and the result replaces has nothing to keep: writing it is no error.
     for (int i = 0; i < count_; ++i)
-      for (uintptr_t t : records(uses_[i])) ensure_f32((const void *)t);
+      for (uintptr_t t : records(uses_[i]))
+        if (!replaces(uses_[i], t)) ensure_f32((const void *)t);
     for (int i = 0; i < count_; ++i)
       if (uses_[i].written)
         for (uintptr_t t : records(uses_[i])) mark_f32((void *)t);
@@ -108,10 +111,14 @@ class Call {
   struct Use {
     const void *p;
     int64_t bytes;
-    bool written;
+    bool written, whole;
   };
   static std::vector<uintptr_t> records(const Use &u) { return reg_within(u.p, (size_t)u.bytes); }
-  int use(const void *p, int64_t bytes, size_t align, bool written) {
+  static bool replaces(const Use &u, uintptr_t t) {
+    const TensorRec *rec = reg_find((const void *)t);
+    return u.whole && rec && rec->fmt == FMT_ELIDED && t >= (uintptr_t)u.p && t + rec->bytes <= (uintptr_t)u.p + (uintptr_t)u.bytes;
+  }
+  int use(const void *p, int64_t bytes, size_t align, bool written, bool whole) {
     if (!p) return 0;
     if ((uintptr_t)p % align) return refuse(BAD_ARGUMENT, who_, "an address is not a multiple of %zu bytes", align);
     cudaPointerAttributes at;
@@ -121,7 +128,7 @@ class Call {
     }
     if (at.type != cudaMemoryTypeManaged && (at.type != cudaMemoryTypeDevice || at.device != device_))
       return refuse(BAD_POINTER, who_, "an address is not memory of the current device");
-    uses_[count_++] = {p, bytes, written};
+    uses_[count_++] = {p, bytes, written, whole};
     return 0;
   }
   bool capturing() const {
@@ -201,7 +208,7 @@ int product(Call &call, ProductArgs &p, cudaStream_t stream) {
   TRY(call.in(p.bias, mats * p.N * 4, 4));
   TRY(call.in(p.index, p.rows * 4, 4));
   TRY(call.in(p.offsets, (p.groups + 1) * 4, 4));
-  TRY(call.out(p.out, span(p.rows, p.ldo, p.N, elem_size(p.out_type)), elem_size(p.out_type)));
+  TRY(call.out(p.out, span(p.rows, p.ldo, p.N, elem_size(p.out_type)), elem_size(p.out_type), p.ldo == p.N));
   p.err = rt().dev_err;
   TRY(call.begin());
   return call.end(launch_product(p, call.num_sms(), stream));
@@ -227,7 +234,7 @@ int occamy_quantize_e4m3(const void *x, int xType, int64_t xRows, int64_t cols, 
   TRY(call.open());
   TRY(call.in(x, span(xRows, ldx, cols, elem_size(xType)), elem_size(xType)));
   TRY(call.in(index, rows * 4, 4));
-  TRY(call.out(q, span(rows, ldq, cols, 1), 1));
+  TRY(call.out(q, span(rows, ldq, cols, 1), 1, ldq == cols));
   TRY(call.out(scales, (rows + blockRows - 1) / blockRows * scale_blocks(cols) * 4, 4));
   TRY(call.begin());
   QuantArgs a = {x, xType, xRows, cols, ldx, index, rows, (int)blockRows, (uint8_t *)q, ldq, scales};
@@ -337,7 +344,7 @@ int occamy_combine_experts(const void *y, int type, int64_t yRows, int64_t ldy, 
   if (yRows) TRY(call.in(y, span(yRows, ldy, N, elem_size(type)), elem_size(type)));
   TRY(call.in(position, tokens * k * 4, 4));
   TRY(call.in(weights, tokens * k * 4, 4));
-  TRY(call.out(out, span(tokens, ldo, N, elem_size(outType)), elem_size(outType)));
+  TRY(call.out(out, span(tokens, ldo, N, elem_size(outType)), elem_size(outType), ldo == N));
   TRY(call.begin());
   CombineArgs a = {y, type, yRows, ldy, position, weights, tokens, k, N, out, outType, ldo};
   return call.end(launch_combine(a, call.num_sms(), stream));

@@ -154,3 +154,37 @@ def test_results_that_span_several_tensors():
             r = f.relu(y, SHAPE)
             assert np.array_equal(f.get(r, SHAPE), np.maximum(z[1], 0))
         del kept
+
+
+def test_results_over_a_tensor_that_fusion_skipped():
+    """conv -> ReLU as one kernel leaves the convolution's own result unwritten; a call may write that tensor all the same."""
+    x, w, b, z = rand(1, *SHAPE), rand(2, 16, 16, 3, 3, scale=0.1), rand(3, 16), rand(4, *SHAPE)
+    src = torch.from_numpy(z.reshape(16, 144)).cuda()
+    stream = torch.cuda.Stream()
+    want = ref.conv2d(x, w, b, (1, 1), act=1)
+    chains = rt.lib().occamy_fused_chains()
+    for i in range(3):
+        with Inference() as f:
+            y, _ = f.conv(f.put(x), SHAPE, f.put(w), w.shape, f.put(b), (1, 1), act=5)
+            r = f.relu(y, SHAPE)
+            if i == 2:
+                kept = copy_rows(src, y, stream)
+                assert np.array_equal(f.get(y, SHAPE), z)
+            assert max_rel_err(f.get(r, SHAPE), want) <= 2e-2
+    assert rt.lib().occamy_fused_chains() > chains
+    del kept
+
+
+def test_a_part_of_a_tensor_that_fusion_skipped_is_not_written():
+    """What the call leaves as it was is not there: reported, as a read would be."""
+    x, w, b = rand(1, *SHAPE), rand(2, 16, 16, 3, 3, scale=0.1), rand(3, 16)
+    src = torch.ones(15, 144, device="cuda")
+    stream = torch.cuda.Stream()
+    for i in range(3):
+        with Inference() as f:
+            y, _ = f.conv(f.put(x), SHAPE, f.put(w), w.shape, f.put(b), (1, 1), act=5)
+            f.get(f.relu(y, SHAPE), SHAPE)
+            if i == 2:
+                kept = copy_rows(src, y, stream)
+    assert rt.last_error(clear=True) == 990
+    del kept
