@@ -268,12 +268,13 @@ int64_t occamy_noalloc_capacity(void);
  * that go to different matrices, and what an expert layer needs around them.  Rules for all of them:
  *   - tensors are row-major; `ld...` is the distance between rows, in elements.  Element types: 0 fp32, 1 bf16, 2 fp16,
  *     3 e4m3 (8-bit floating point, largest value 448, no infinity).
- *   - every pointer is memory of the CURRENT device, results overlap no input, and work is enqueued on `stream`, a stream of
- *     that device; nothing waits and nothing is allocated, so calls can be captured into a graph, all but the process's first
- *     (refused with -6; it sets the runtime up).  `stream` may be any,
- *     occamy_stream() among them.  Memory that came from wrapDNNMalloc or a pool is brought up to date first (a result
- *     that a convolution left in another format, for instance) and ordered with the runtime's own stream on both sides;
- *     while `stream` is captured such memory is refused (-6), unless `stream` is occamy_stream().
+ *   - every pointer is memory of the CURRENT device, results overlap no input, and work is enqueued on `stream`, a
+ *     stream of that device (any, occamy_stream() among them); nothing waits and nothing is allocated, so calls can be
+ *     captured into a graph, all but the process's first (refused with -6; it sets the runtime up).
+ *   - memory that came from wrapDNNMalloc or a pool may be used too: all tensors that an operand reaches into are
+ *     brought up to date first (a result that a convolution left in another format, for instance, which may wait and
+ *     allocate) and ordered with the runtime's own stream on both sides.  In a capture such memory is refused (-6):
+ *     while `stream` is captured, and while occamy_stream() is.
  *   - results have the same bits from call to call; elements of a result's rows behind its columns, and rows
  *     that no group or index reaches, are left as they were.  Sums are held in fp32.
  *   - returns 0 (also for an empty problem, which launches nothing), a negative code with a line on stderr and nothing

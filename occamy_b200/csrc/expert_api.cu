@@ -59,11 +59,11 @@ class Call {
     // the runtime's state is set up by the first call of any kind, which a stream that is captured does not allow
     static bool ready = false;
     if (!ready) {
-      if (capturing()) return refuse(CAPTURED, who_, "the first call cannot be captured");
+      if (capturing(stream_)) return refuse(CAPTURED, who_, "the first call cannot be captured");
       rt();
       ready = true;
     }
-    if (stream_ == rt().stream) {
+    if (stream_ == rt().stream && !capturing(stream_)) {   // (what is put off is no part of the caller's graph)
       occamy_internal_opaque_call();
       settled_ = true;
     }
@@ -80,8 +80,9 @@ class Call {
     // (a tensor of an inference that is being replayed is not on record until its calls are made one by one)
     for (int i = 0; i < count_ && !tracked; ++i) tracked = in_live_pool(uses_[i].p) || !records(uses_[i]).empty();
     if (!tracked) return 0;
-    if (stream_ != rt().stream && capturing())
-      return refuse(CAPTURED, who_, "memory of the runtime's own cannot be used while the stream is captured");
+    // Bringing it up to date would be done by every replay, or not at all, and a replay cannot put on record what it wrote.
+    if (capturing(stream_) || capturing(rt().stream))
+      return refuse(CAPTURED, who_, "memory of the runtime's own cannot be used while the stream, or occamy_stream(), is captured");
     if (!settled_) occamy_internal_opaque_call();
     tracked_ = true;
     // A result may leave parts of its memory as they were: they have to be there too.  (An operand may be several tensors.)
@@ -131,9 +132,9 @@ class Call {
     uses_[count_++] = {p, bytes, written, whole};
     return 0;
   }
-  bool capturing() const {
+  static bool capturing(cudaStream_t s) {
     cudaStreamCaptureStatus st = cudaStreamCaptureStatusNone;
-    if (cudaStreamIsCapturing(stream_, &st) == cudaSuccess && st == cudaStreamCaptureStatusNone) return false;
+    if (cudaStreamIsCapturing(s, &st) == cudaSuccess && st == cudaStreamCaptureStatusNone) return false;
     cudaGetLastError();
     return true;
   }

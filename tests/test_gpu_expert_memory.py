@@ -188,3 +188,38 @@ def test_a_part_of_a_tensor_that_fusion_skipped_is_not_written():
                 kept = copy_rows(src, y, stream)
     assert rt.last_error(clear=True) == 990
     del kept
+
+
+def test_captures_of_the_runtimes_stream():
+    """Memory of the runtime's own is refused in a capture, of its stream too: what has to happen to it first would become part of
+    the graph, and a replay could not tell the runtime what it wrote.  Other memory is captured there like anywhere."""
+    x = rand(1, 16, 256)
+    fresh, plain = rt.DeviceBuffer(x.nbytes), rt.DeviceBuffer.from_numpy(x)
+    rt.synchronize()
+    xt = torch.zeros(16, 256, device="cuda")
+    q = torch.zeros(16, 256, dtype=torch.uint8, device="cuda").view(torch.float8_e4m3fn)
+    scales = torch.zeros(16, 2, device="cuda")
+    own = torch.cuda.ExternalStream(rt.lib().occamy_stream())
+    other = torch.cuda.Stream()
+
+    def call(p, s, out=None):
+        return rt.lib().occamy_quantize_e4m3(p, rt.F32, 16, 256, 256, None, 16, 1, out or q.data_ptr(), 256, scales.data_ptr(),
+                                             s.cuda_stream)
+    assert call(xt.data_ptr(), own) == 0
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g, stream=own):
+        codes = [call(fresh.ptr, own), call(plain.ptr, own), call(xt.data_ptr(), own, fresh.ptr), call(plain.ptr, other),
+                 call(xt.data_ptr(), own)]
+    assert codes == [-6, -6, -6, -6, 0]
+    for i in range(3):
+        x = rand(10 + i, 16, 256)
+        xt.copy_(torch.from_numpy(x))
+        torch.cuda.synchronize()
+        g.replay()
+        same_quantised((q, scales), x)
+    # nothing that is put off has been done, or noted as done, meanwhile
+    assert call(fresh.ptr, other) == 0
+    same_quantised((q, scales), np.zeros((16, 256), np.float32))
+    fresh.free()
+    plain.free()
