@@ -95,13 +95,13 @@ class Call {
         for (uintptr_t t : records(uses_[i])) mark_f32((void *)t);
     return stream_ == rt().stream ? 0 : order(rt().stream, stream_);
   }
-  // `e`: of the launches.
-  int end(cudaError_t e) {
+  // `e`: of the launches, of so many kernels.
+  int end(cudaError_t e, int kernels = 1) {
     if (e != cudaSuccess) {
       cudaGetLastError();
       return refuse((int)e, who_, "%s", cudaGetErrorString(e));
     }
-    count(CNT_LAUNCHES, 1);
+    count(CNT_LAUNCHES, kernels);
     if (!tracked_ || stream_ == rt().stream) return 0;
     return order(stream_, rt().stream);
   }
@@ -313,7 +313,8 @@ int occamy_route_experts(const void *logits, int type, int64_t tokens, int64_t e
   TRY(call.out(offsets, (experts + 1) * 4, 4));
   if (tokens == 0) {
     TRY(call.begin());
-    return call.end(cudaMemsetAsync(offsets, 0, (size_t)(experts + 1) * 4, stream));
+    rt().main_copies++;   // (that a later upload goes behind it: wrapDNNMemcpy)
+    return call.end(cudaMemsetAsync(offsets, 0, (size_t)(experts + 1) * 4, stream), 0);
   }
   TRY(call.in(logits, span(tokens, ldl, experts, elem_size(type)), elem_size(type)));
   TRY(call.out(chosen, tokens * k * 4, 4));
@@ -324,7 +325,7 @@ int occamy_route_experts(const void *logits, int type, int64_t tokens, int64_t e
   TRY(call.begin());
   RouteArgs a = {logits, type, tokens, experts, ldl, (int)k, normalise != 0, chosen, weights, offsets, order, position,
                  (int32_t *)workspace};
-  return call.end(launch_route(a, stream));
+  return call.end(launch_route(a, stream), route_kernels(tokens));
 } catch (...) {
   return FAILED;
 }

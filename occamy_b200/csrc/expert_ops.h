@@ -73,6 +73,7 @@ cudaError_t launch_quantize_e4m3(const QuantArgs &a, int num_sms, cudaStream_t s
 cudaError_t launch_product(const ProductArgs &a, int num_sms, cudaStream_t s);
 cudaError_t launch_route(const RouteArgs &a, cudaStream_t s);
 size_t route_workspace(int64_t tokens, int64_t experts, int64_t k);
+int route_kernels(int64_t tokens);   // that launch_route() launches
 cudaError_t launch_combine(const CombineArgs &a, int num_sms, cudaStream_t s);
 
 #ifdef OCCAMY_TC_TIMERS

@@ -501,6 +501,8 @@ size_t route_workspace(int64_t tokens, int64_t experts, int64_t) {
   return (size_t)((tokens + per - 1) / per) * (size_t)experts * 4;
 }
 
+int route_kernels(int64_t tokens) { return tokens <= tokens_of_block(tokens) ? 1 : 2; }
+
 cudaError_t launch_route(const RouteArgs &a, cudaStream_t s) {
   if (a.type == ELEM_F32) return launch_route_typed<float>(a, s);
   if (a.type == ELEM_BF16) return launch_route_typed<__nv_bfloat16>(a, s);

@@ -223,3 +223,11 @@ def test_captures_of_the_runtimes_stream():
     same_quantised((q, scales), np.zeros((16, 256), np.float32))
     fresh.free()
     plain.free()
+
+
+@pytest.mark.parametrize("tokens,launches", [(0, 0), (1, 1), (128, 1), (129, 2), (5000, 2)])
+def test_launches_of_routing_are_counted(tokens, launches):
+    logits = torch.randn(tokens, 16, device="cuda")
+    before = rt.counters()["launches"]
+    assert ec.route(logits, 2, True)[0] == 0
+    assert rt.counters()["launches"] - before == launches
