@@ -208,7 +208,8 @@ void occamy_get_counters(int64_t out[8]);
  * 2x2 max pool along, [4] inferences whose recorded part ran as graphs, [5] such that were computed in
  * pieces while their batch arrived, [6] convolutions that took another one's result along as a second
  * summand, [7] pairs of layers as one kernel, [8] few-channel convolutions that read whole input rows, [9] to [12]
- * occamy_matmul_e4m3 / _grouped calls in tiles of 32, 64, 128 and 256 rows.  Returns how many there are. */
+ * occamy_matmul_e4m3 / _grouped calls in tiles of 32, 64, 128 and 256 rows, [13] those whose tiles' K clusters share.
+ * Returns how many there are. */
 int occamy_get_form_counters(int64_t *out, int n);
 /* Per-launch timing of the tensor-core convolution / GEMM kernel: after _begin, every such
  * launch is bracketed by a CUDA-event pair on the launch stream; _end waits for the stream,

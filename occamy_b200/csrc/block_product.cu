@@ -595,6 +595,7 @@ cudaError_t launch_tiles(PtParams &p, int64_t most_tiles, int num_sms, cudaStrea
 #ifdef OCCAMY_TUNING
   if (const char *e = getenv("OCCAMY_PT_SPLITS")) p.splits = atoi(e);
 #endif
+  if (p.splits > 1) count(CNT_PRODUCT_SHARED);
   const int64_t grid = p.splits > 1 ? most_tiles * p.splits : std::min<int64_t>(most_tiles, resident);
   return launch_after(block_product_kernel<BN, SCALED, GATED>, dim3((unsigned)grid), dim3(PT_THREADS), smem, s,
                       p.splits, p);

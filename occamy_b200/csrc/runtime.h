@@ -91,7 +91,8 @@ enum Counter {
   CNT_PAIRS = 15,
   CNT_ROWS = 16,
   CNT_PRODUCT_32 = 17,   // and three more: tiles of 64, 128, 256 rows
-  CNT_COUNT = 21
+  CNT_PRODUCT_SHARED = 21,   // calls whose tiles' K clusters share
+  CNT_COUNT = 22
 };
 
 struct Runtime {

@@ -183,6 +183,14 @@ def form_counters() -> dict:
     return dict(zip(FORM_NAMES, [int(v) for v in out]))
 
 
+def products_with_shared_k() -> int:
+    """Calls of the 8-bit and grouped products whose tiles' K clusters share (a form besides those of form_counters())."""
+    n = len(FORM_NAMES) + 1
+    out = (C.c_int64 * n)()
+    lib().occamy_get_form_counters(out, n)
+    return int(out[-1])
+
+
 class DeviceBuffer:
     """A device allocation from the ABI's allocator (zero-filled, as the ABI promises)."""
 
