@@ -291,19 +291,22 @@ int64_t occamy_noalloc_capacity(void);
 int occamy_quantize_e4m3(const void *x, int xType, int64_t xRows, int64_t cols, int64_t ldx,
                          const int32_t *index, int64_t rows, int64_t blockRows, void *q, int64_t ldq,
                          float *scales, cudaStream_t stream);
-/* out[M][N] = act(A B^T + bias) of e4m3 A[M][K] and B[N][K]: the value of A[m][k] is a * scaleA[m][k / 128], that of B[n][k]
- * b * scaleB[n / 128][k / 128]; both scale arrays are dense, of any fp32 numbers.  bias [N] or null, fp32.  activMode as in
- * DNNConvBiasActivFunc and DNNActiveFunc, 0 sigmoid, 1 ReLU, 2 tanh, 3 clip to [0, 6], 5 identity, and 6: x * sigmoid(x).
- * outType 0, 1 or 2.  A and B start at multiples of 16 bytes, and so do their rows (lda % 16 == 0, ldb % 16 == 0).  M and N (below:
- * rows, and rows of all matrices of B) are at most 2^31 - 1024. */
+/* out[M][N] = act(A B^T + bias) of e4m3 A[M][K] and B[N][K]: the value of A[m][k] is a * scaleA[m][k / 128], that of
+ * B[n][k] b * scaleB[n / 128][k / 128].  Both scale arrays are dense, of any fp32 numbers, and the product of two of them
+ * need not be one.  (Only where either is 2^-126, as for a block of zeros, a product below 2^-126 is rounded to a multiple
+ * of 2^-149.)  bias [N] or null, fp32.  activMode as in DNNConvBiasActivFunc and DNNActiveFunc, 0 sigmoid, 1 ReLU, 2 tanh,
+ * 3 clip to [0, 6], 5 identity, and 6: x * sigmoid(x).  outType 0, 1 or 2.  A and B start at multiples of 16 bytes, and so
+ * do their rows (lda % 16 == 0, ldb % 16 == 0).  M and N (below: rows, and rows of all matrices of B) are at most
+ * 2^31 - 1024. */
 int occamy_matmul_e4m3(const void *a, int64_t lda, const float *scaleA, const void *b, int64_t ldb,
                        const float *scaleB, const float *bias, int64_t M, int64_t N, int64_t K,
                        int64_t activMode, void *out, int outType, int64_t ldo, cudaStream_t stream);
 /* The same for rows in groups: rows offsets[g] .. offsets[g + 1] - 1 of out are the rows of A times matrix g of B.
- * offsets: groups + 1 numbers in device memory, ascending, cut off at [0, rows] (one below an earlier one counts as that); rows in
- * front of the first and behind the last are left as they were.  Row i is row index[i] of A[aRows][K], one outside [0, aRows) counts as zeros (index null: row i, and rows ==
- * aRows; with one, A has at most 64 GiB).  type 1 or 2: A and B are bf16 / fp16 and have no scales; type 3: as above, with scaleB [groups][ceil(N / 128)]
- * [ceil(K / 128)].  B: [groups][N][K], rows ldb apart, bias: [groups][N] or null.  Up to 1024 groups.
+ * offsets: groups + 1 numbers in device memory, ascending, cut off at [0, rows] (one below an earlier one counts as that);
+ * rows in front of the first and behind the last are left as they were.  Row i is row index[i] of A[aRows][K], one outside
+ * [0, aRows) counts as zeros (index null: row i, and rows == aRows; with one, A has at most 64 GiB).  type 1 or 2: A and B
+ * are bf16 / fp16 and have no scales, and their rows start at multiples of 16 bytes too; type 3: as above, with scaleB
+ * [groups][ceil(N / 128)][ceil(K / 128)].  B: [groups][N][K], rows ldb apart, bias: [groups][N] or null.  Up to 1024 groups.
  * activMode 7: out = silu(first) * second of two matrices for each group; then B is [groups][2][N][K], scaleB and bias have
  * that 2 as well, and N % 8 == 0. */
 int occamy_matmul_grouped(const void *a, int type, int64_t aRows, int64_t lda, const float *scaleA,

@@ -40,7 +40,8 @@ __global__ void __launch_bounds__(PT_THREADS, BN <= 64 ? 2 : 1) block_product_ke
   constexpr int EW = PT_EPI_WARPS;
   constexpr int CW = BN / (EW / 4);      // columns of an epilogue warp
   constexpr int NG = CW / 8;             // groups of eight of them
-  constexpr int LD = CW < 32 ? CW : 32;  // columns of one TMEM load
+  // Columns of one TMEM load.  (Of 64 columns 16: with 32 the code around the sums decided whether 256 x 4096 x 25088 took 50 or 58 us.)
+  constexpr int LD = CW < 32 || BN == 128 ? 16 : 32;
   constexpr int SETS = GATED ? 2 : 1;    // scales of a column: first and second matrix
   constexpr int TILE_N = GATED ? PT_ROWS / 2 : PT_ROWS;
   extern __shared__ __align__(1024) uint8_t smem_raw[];
@@ -65,6 +66,12 @@ __global__ void __launch_bounds__(PT_THREADS, BN <= 64 ? 2 : 1) block_product_ke
   volatile uint32_t *tmem_holder = reinterpret_cast<volatile uint32_t *>(words);
   volatile int *abort_flag = words + 1;
   const PtGroups groups = {words + 4, words + 4 + p.groups, words + 4 + 2 * p.groups};
+  // of each buffer, for factors out of range: the powers that go with them ([SETS][BN]), whether a scale warp wants them applied, and a
+  // barrier for the answer
+  float *powers = reinterpret_cast<float *>(smem_raw + ((reinterpret_cast<uint8_t *>(words + 5 + 3 * p.groups) - smem_raw + 15) & ~15));
+  volatile int *wanted = reinterpret_cast<volatile int *>(powers + bufs * SETS * BN);
+  const uint32_t applied0 = smem_u32(powers + bufs * SETS * BN + 2 * bufs);
+  auto applied_bar = [&](int b, int w) { return applied0 + 8u * (2 * b + w); };
 
   const int warp = warp_index(), lane = threadIdx.x & 31;
   const bool indexed = BN < 256 && p.index;   // (choose_rows)
@@ -80,6 +87,11 @@ __global__ void __launch_bounds__(PT_THREADS, BN <= 64 ? 2 : 1) block_product_ke
       mbar_init(tfull_bar(b), 1);
       mbar_init(tempty_bar(b), EW);
       mbar_init(sfull_bar(b), 2);
+      if constexpr (SCALED)
+        for (int w = 0; w < 2; ++w) {
+          mbar_init(applied_bar(b, w), EW);
+          wanted[2 * b + w] = 0;
+        }
     }
     *abort_flag = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -272,7 +284,7 @@ __global__ void __launch_bounds__(PT_THREADS, BN <= 64 ? 2 : 1) block_product_ke
       constexpr int MINE = BN <= 64 ? 1 : BN / 64;
       const int t = threadIdx.x - 64;
       int buf = 0;
-      uint32_t buf_phase = 0;
+      uint32_t buf_phase = 0, applied = 0;   // (a phase for each buffer)
       for (int tile = tile0; tile < total && !err_code; tile += tstep) {
         const PtTile tl = decode(tile);
         const float *sa[MINE];
@@ -285,17 +297,25 @@ __global__ void __launch_bounds__(PT_THREADS, BN <= 64 ? 2 : 1) block_product_ke
         const float *sb = p.scale_b + ((int64_t)tl.g * SETS * p.blocks_n + tl.n0 / SCALE_BLOCK) * p.kblocks;
         const int64_t second = (int64_t)p.blocks_n * p.kblocks;
         float va[MINE][4], vb[SETS][4];
-        auto fetch = [&](int kq) {
+        auto fetch = [&](int kq) {   // 1 where there is none (the numbers of a row that an index does not give are zeros)
 #pragma unroll
           for (int j = 0; j < 4; ++j) {
 #pragma unroll
-            for (int i = 0; i < MINE; ++i) va[i][j] = sa[i] && kq + j < k1 ? __ldg(sa[i] + kq + j) : 0.0f;
+            for (int i = 0; i < MINE; ++i) va[i][j] = sa[i] && kq + j < k1 ? __ldg(sa[i] + kq + j) : 1.0f;
 #pragma unroll
-            for (int h = 0; h < SETS; ++h) vb[h][j] = kq + j < k1 ? __ldg(sb + h * second + kq + j) : 0.0f;
+            for (int h = 0; h < SETS; ++h) vb[h][j] = kq + j < k1 ? __ldg(sb + h * second + kq + j) : 1.0f;
           }
         };
         fetch(k0);
         for (int kq = k0; kq < k1 && !err_code; kq += 4) {
+          uint32_t range = 0;   // of these four
+#pragma unroll
+          for (int j = 0; j < 4; ++j)
+#pragma unroll
+            for (int i = 0; i < MINE; ++i)
+#pragma unroll
+              for (int h = 0; h < SETS; ++h) range = max(range, pt_range(va[i][j], vb[h][j]));
+          const bool look = __any_sync(0xffffffffu, range > PT_RANGE);
 #pragma unroll
           for (int j = 0; j < 4; ++j) {
             if (kq + j >= k1 || err_code) continue;
@@ -309,6 +329,32 @@ __global__ void __launch_bounds__(PT_THREADS, BN <= 64 ? 2 : 1) block_product_ke
 #pragma unroll
               for (int h = 0; h < SETS; ++h)
                 if (BN >= 64 || t < BN) dst[h * BN + 64 * i] = va[i][j] * vb[h][j];
+            if (look) {
+              bool met = false;
+              float *pow = powers + buf * (SETS * BN) + t;
+#pragma unroll
+              for (int i = 0; i < MINE; ++i)
+#pragma unroll
+                for (int h = 0; h < SETS; ++h) {
+                  float f;
+                  const float power = pt_factor(va[i][j], vb[h][j], f);
+                  met = met || power != 1.0f;
+                  if (BN >= 64 || t < BN) dst[h * BN + 64 * i] = f, pow[h * BN + 64 * i] = power;
+                }
+              if (__any_sync(0xffffffffu, met)) {
+                // The sums' warps find this while they wait for the scales, which do not arrive before it is done; their loop does not look
+                // for it.  (A word read in every k-step took 256 x 4096 x 25088 from 50 us to 52 at best, 60 at worst.)
+                __threadfence_block();
+                __syncwarp();
+                if (lane == 0) wanted[2 * buf + warp - 2] = 1;
+                if (!mbar_wait_warp(applied_bar(buf, warp - 2), applied >> buf & 1u, abort_flag)) {
+                  err_code = 6;
+                  continue;
+                }
+                applied ^= 1u << buf;
+                if (lane == 0) wanted[2 * buf + warp - 2] = 0;
+              }
+            }
             __syncwarp();
             if (lane == 0) mbar_arrive(sfull_bar(buf));
             if (++buf == bufs) {
@@ -333,6 +379,38 @@ __global__ void __launch_bounds__(PT_THREADS, BN <= 64 ? 2 : 1) block_product_ke
     else if constexpr (BN == 256) asm volatile("setmaxnreg.inc.sync.aligned.u32 200;");
     else asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
     TCT_DECL
+    // For a buffer's scales; applies the powers that a scale warp wants before they arrive, to its 32 columns of every 64.
+    auto wait_scales = [&](const PtTile &tl, int buf, uint32_t phase) {
+      if (__all_sync(0xffffffffu, mbar_try(sfull_bar(buf), phase))) return true;
+      const long long t0 = clock64();
+      int done = 0;
+      for (int it = 1; !__all_sync(0xffffffffu, mbar_try(sfull_bar(buf), phase)); ++it) {
+        for (int w = 0; w < 2; ++w) {
+          if (done >> w & 1 || !__shfl_sync(0xffffffffu, wanted[2 * buf + w], 0)) continue;
+          __threadfence_block();
+          if (!mbar_wait_warp(tfull_bar(buf), phase, abort_flag)) return false;
+          tc_fence_after();
+          if (c0 < tl.rows) {
+            const int at = buf * (SETS * BN) + (GATED ? ((lane >> 3) & 1) * BN : 0) + c0;
+#pragma unroll 1
+            for (int s = 0; s < CW; s += 16)
+              if (((c0 + s) / 32 & 1) == w) pt_rescale(tmem + ((uint32_t)(quad * 32) << 16) + (uint32_t)(buf * BN + c0 + s), powers + at + s);
+            asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+          }
+          done |= 1 << w;
+          __syncwarp();
+          if (lane == 0) mbar_arrive(applied_bar(buf, w));
+        }
+        if ((it & 15) == 0) {
+          const bool late = clock64() - t0 > 4000000000LL;
+          if (__any_sync(0xffffffffu, *abort_flag != 0 || late)) {
+            if (late) *abort_flag = 1;
+            return false;
+          }
+        }
+      }
+      return true;
+    };
     uint64_t acc[CW / 2];                  // sums of weight `lane` of the quadrant and columns c0 + 2 i, 2 i + 1
     int buf = 0;
     uint32_t buf_phase = 0;
@@ -343,7 +421,7 @@ __global__ void __launch_bounds__(PT_THREADS, BN <= 64 ? 2 : 1) block_product_ke
 #pragma unroll
       for (int i = 0; i < CW / 2; ++i) acc[i] = 0;
       for (int kb = k0; kb < k1; kb += PER) {
-        if (SCALED && !TCT_WAIT(0, mbar_wait_warp(sfull_bar(buf), buf_phase, abort_flag))) {
+        if (SCALED && !TCT_WAIT(0, wait_scales(tl, buf, buf_phase))) {
           err_code = 5;
           break;
         }
@@ -576,7 +654,7 @@ cudaError_t launch_tiles(PtParams &p, int64_t most_tiles, int num_sms, cudaStrea
   constexpr size_t LIMIT = BN <= 64 ? TC_SMEM_DUO : TC_SMEM_LIMIT;
   constexpr int EW = PT_EPI_WARPS;
   p.bufs = BN == 256 ? 2 : 4;
-  const size_t misc = EW * 1024 + (SCALED ? p.bufs * (GATED ? 2 : 1) * BN * 4 : 0) + 8 * 3 * 4 + 16 +
+  const size_t misc = EW * 1024 + (SCALED ? p.bufs * ((GATED ? 2 : 1) * BN * 8 + 24) + 16 : 0) + 8 * 3 * 4 + 16 +
                       (3 * (size_t)p.groups + 1) * 4;
   const size_t stage = (PT_ROWS + BN) * 128 + 16;
   p.stages = (int)std::min<size_t>((LIMIT - misc) / stage, 16);

@@ -77,6 +77,63 @@ __device__ __forceinline__ void load_5d_warp(uint32_t dst, const CUtensorMap *m,
       : "memory");
 }
 
+// Waits for a thread's TMEM loads; the values are not to be used before.
+template <int V>
+__device__ __forceinline__ void pt_ld_wait(uint32_t *v) {
+  asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+#pragma unroll
+  for (int i = 0; i < V; ++i) asm volatile("" : "+r"(v[i])::"memory");
+}
+
+// ---- scales
+// A k-step's sums v (0, or 2^-18 to 2^25) are multiplied by sA * sB, which fp32 does not hold for all scales although v sA sB fits: 2^-75
+// and 2^-75 would give 0, 2^64 and 2^64 infinity, and NaN where v is 0.  Such a factor is kept as f 2^p instead, p = -96 below
+// 2^-126 (unless fp32 has that number) and 64 from 2^128 on, where f is in range or far enough out of it; v 2^p is exact, and v 2^p f
+// rounded once.  That is rare: the exponents say whether any of four k-steps may be so, which is looked at then alone.  (One factor is
+// left as fp32 rounds it, to a multiple of 2^-149: that of the scale 2^-126, a block of zeros or of numbers below 2^-117.  Padded rows
+// have nothing else, and what is lost is below 2^-125.)
+constexpr float PT_DOWN = 1.262177448e-29f, PT_UP = 18446744073709551616.0f;   // 2^-96, 2^64
+// Above PT_RANGE where a * b may not be a normal number (by the exponents; also where either is 0 or subnormal) and a is not 2^-126.
+constexpr uint32_t PT_RANGE = 250u << 23;
+__device__ __forceinline__ uint32_t pt_range(float a, float b) {
+  const uint32_t u = __float_as_uint(a), e = u == 0x00800000u ? 127u << 23 : u & 0x7f800000u;
+  return e + (__float_as_uint(b) & 0x7f800000u) - (129u << 23);
+}
+// f = sA * sB or as above; returns 2^p.
+__device__ __forceinline__ float pt_factor(float a, float b, float &f) {
+  const float most = 3.402823466e38f;
+  f = a * b;
+  const float m = fabsf(f);
+  if ((m >= 1.175494351e-38f && m <= most) || a == 0.0f || b == 0.0f || !(fabsf(a) <= most) || !(fabsf(b) <= most)) return 1.0f;
+  if (m < 1.0f) {
+    if (a == 1.175494351e-38f || b == 1.175494351e-38f) return 1.0f;
+    const float g = (a * 281474976710656.0f) * (b * 281474976710656.0f);   // 2^48
+    if (f * 79228162514264337593543950336.0f == g) return 1.0f;            // 2^96
+    f = g;
+    return PT_DOWN;
+  }
+  f = fminf(fmaxf((a * 2.328306437e-10f) * (b * 2.328306437e-10f), -most), most);   // 2^-32
+  return PT_UP;
+}
+
+// This warp's TMEM lanes, 16 columns from `from` on: times `power`, a number for each column.
+__device__ __forceinline__ void pt_rescale(uint32_t from, const float *power) {
+  uint32_t v[16];
+  tc_ld<16>(from, v);
+  pt_ld_wait<16>(v);
+#pragma unroll
+  for (int i = 0; i < 16; i += 2) {
+    const float2 w = *reinterpret_cast<const float2 *>(power + i);
+    v[i] = __float_as_uint(__uint_as_float(v[i]) * w.x);
+    v[i + 1] = __float_as_uint(__uint_as_float(v[i + 1]) * w.y);
+  }
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};" ::"r"(from),
+      "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(v[8]), "r"(v[9]), "r"(v[10]),
+      "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15])
+      : "memory");
+}
+
 // ---- rows chosen by an index
 // Four warps copy them, 16 bytes a lane, in the swizzled order that the tensor core reads.  (TMA's own gather of four rows
 // takes 75 cycles an instruction, 2400 for the 128 rows of a k-step; a cp.async of a warp takes that warp 30 cycles, a k-step

@@ -12,6 +12,7 @@
 // both).
 #include <algorithm>
 #include <mutex>
+#include <type_traits>
 
 #include "block_product_dev.cuh"
 
@@ -23,14 +24,8 @@ constexpr int PW_COLUMNS = PW_WEIGHTS / (PT_EPI_WARPS / 4);   // of an epilogue 
 constexpr int PW_STAGE_OUT = 1024;                  // of each epilogue warp: 32 rows x 32 bytes
 constexpr int PW_BATCH = 4;                         // k-steps whose scales come together
 constexpr int PW_SCALES = PW_BATCH * 2 * 128;       // of a slot: [k-step][half of the tile's weights, or matrix][row]
+constexpr int PW_SLOT = 2 * PW_SCALES * 4 + 8;      // bytes, with what goes with factors out of range, and whether there are any
 
-// Waits for a thread's TMEM loads; the values are not to be used before.
-template <int V>
-__device__ __forceinline__ void pw_wait(uint32_t *v) {
-  asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
-#pragma unroll
-  for (int i = 0; i < V; ++i) asm volatile("" : "+r"(v[i])::"memory");
-}
 template <bool GATED>
 __global__ void __launch_bounds__(PT_THREADS, 1) block_product_wide_kernel(const __grid_constant__ PtParams p) {
   constexpr int SETS = GATED ? 2 : 1;
@@ -46,7 +41,9 @@ __global__ void __launch_bounds__(PT_THREADS, 1) block_product_wide_kernel(const
   const uint32_t sA = smem_u32(smem_raw), sB = sA + stages * A_BYTES;
   uint8_t *stage_out = smem_raw + stages * (A_BYTES + B_BYTES);
   float *scales = reinterpret_cast<float *>(stage_out + PT_EPI_WARPS * PW_STAGE_OUT);   // two slots
-  uint64_t *bars = reinterpret_cast<uint64_t *>(scales + 2 * PW_SCALES);
+  float *powers = scales + 2 * PW_SCALES;
+  uint2 *any_power = reinterpret_cast<uint2 *>(powers + 2 * PW_SCALES);   // of either scale warp
+  uint64_t *bars = reinterpret_cast<uint64_t *>(any_power + 2);
   const uint32_t bar0 = smem_u32(bars);
   auto full_bar = [&](int s) { return bar0 + 8u * s; };
   auto empty_bar = [&](int s) { return bar0 + 8u * (stages + s); };
@@ -198,17 +195,25 @@ __global__ void __launch_bounds__(PT_THREADS, 1) block_product_wide_kernel(const
         sb[h] = p.scale_b + ((int64_t)tl.g * SETS * p.blocks_n + block) * kblocks;
       }
       float va[2][PW_BATCH], vb[2][PW_BATCH];
-      auto fetch = [&](int kq) {
+      auto fetch = [&](int kq) {   // 1 where there is none (the numbers of a row that an index does not give are zeros)
 #pragma unroll
         for (int j = 0; j < PW_BATCH; ++j) {
 #pragma unroll
-          for (int i = 0; i < 2; ++i) va[i][j] = sa[i] && kq + j < kblocks ? __ldg(sa[i] + kq + j) : 0.0f;
+          for (int i = 0; i < 2; ++i) va[i][j] = sa[i] && kq + j < kblocks ? __ldg(sa[i] + kq + j) : 1.0f;
 #pragma unroll
-          for (int h = 0; h < 2; ++h) vb[h][j] = kq + j < kblocks ? __ldg(sb[h] + kq + j) : 0.0f;
+          for (int h = 0; h < 2; ++h) vb[h][j] = kq + j < kblocks ? __ldg(sb[h] + kq + j) : 1.0f;
         }
       };
       fetch(0);
       for (int kq = 0; kq < kblocks; kq += PW_BATCH) {
+        uint32_t range = 0;
+#pragma unroll
+        for (int j = 0; j < PW_BATCH; ++j)
+#pragma unroll
+          for (int h = 0; h < 2; ++h)
+#pragma unroll
+            for (int i = 0; i < 2; ++i) range = max(range, pt_range(va[i][j], vb[h][j]));
+        const bool look = __any_sync(0xffffffffu, range > PT_RANGE);
         if (!TCT_WAIT(0, mbar_wait_warp(sempty_bar(slot), slot_phase ^ 1u, abort_flag))) {
           err_code = 4;
           break;
@@ -220,6 +225,23 @@ __global__ void __launch_bounds__(PT_THREADS, 1) block_product_wide_kernel(const
           for (int h = 0; h < 2; ++h)
 #pragma unroll
             for (int i = 0; i < 2; ++i) dst[(j * 2 + h) * 128 + 64 * i] = va[i][j] * vb[h][j];
+        bool met = false;
+        if (look) {
+          float *pow = powers + slot * PW_SCALES + t;
+#pragma unroll
+          for (int j = 0; j < PW_BATCH; ++j)
+#pragma unroll
+            for (int h = 0; h < 2; ++h)
+#pragma unroll
+              for (int i = 0; i < 2; ++i) {
+                float f;
+                const float power = pt_factor(va[i][j], vb[h][j], f);
+                met = met || power != 1.0f;
+                dst[(j * 2 + h) * 128 + 64 * i] = f, pow[(j * 2 + h) * 128 + 64 * i] = power;
+              }
+          met = __any_sync(0xffffffffu, met);
+        }
+        if (lane == 0) reinterpret_cast<uint32_t *>(any_power + slot)[warp - 2] = met;
         __syncwarp();
         if (lane == 0) mbar_arrive(sfull_bar(slot));
         if (++slot == 2) {
@@ -283,18 +305,11 @@ __global__ void __launch_bounds__(PT_THREADS, 1) block_product_wide_kernel(const
             slot_phase ^= 1u;
           }
         };
-        if constexpr (!GATED) {
-#pragma unroll
-          for (int j = 0; j < PW_BATCH; ++j) take(j);
-          taken();
-        }
-#pragma unroll
-        for (int j = 0; j < PW_BATCH; ++j) {
-          if (kq + j >= kblocks || err_code) continue;
-          if constexpr (GATED) take(j);
+        // One k-step: its columns into the sums, each times its factor `w` (odd: times `power` first).
+        auto step = [&](const float *w, auto odd, const float *power) {
           if (!TCT_WAIT(1, mbar_wait_warp(tfull_bar(buf), buf_phase, abort_flag))) {
             err_code = 5;
-            continue;
+            return;
           }
           tc_fence_after();
           const uint32_t from = tmem + ((uint32_t)(quad * 32) << 16) + (uint32_t)(buf * PW_WEIGHTS + c0);
@@ -304,13 +319,18 @@ __global__ void __launch_bounds__(PT_THREADS, 1) block_product_wide_kernel(const
               uint32_t v[V_COLUMNS];
 #pragma unroll
               for (int i = 0; i < V_COLUMNS; i += 32) tc_ld<V_COLUMNS < 32 ? V_COLUMNS : 32>(from + s * V_COLUMNS + i, v + i);
-              pw_wait<V_COLUMNS>(v);
+              pt_ld_wait<V_COLUMNS>(v);
               if (s + 1 == STEPS) {   // all of this buffer has been read
                 tc_fence_before();
                 __syncwarp();
                 if (lane == 0) mbar_arrive(tempty_bar(buf));
               }
-              add(v, s, f[j % AHEAD]);
+              if constexpr (decltype(odd)::value) {
+#pragma unroll
+                for (int i = 0; i < V_COLUMNS; ++i)
+                  v[i] = __float_as_uint(__uint_as_float(v[i]) * power[GATED ? ((s * V_COLUMNS + i) >> 3) & 1 : 0]);
+              }
+              add(v, s, w);
             }
           } else if (lane == 0) {
             mbar_arrive(tempty_bar(buf));
@@ -319,6 +339,33 @@ __global__ void __launch_bounds__(PT_THREADS, 1) block_product_wide_kernel(const
             buf = 0;
             buf_phase ^= 1u;
           }
+        };
+        const uint2 odd = any_power[slot];
+        if (quad & 1 ? odd.y : odd.x) {   // (of the scale warp that has this quadrant's rows)
+#pragma unroll 1
+          for (int j = 0; j < PW_BATCH && kq + j < kblocks && !err_code; ++j) {
+            float w[SETS], power[SETS];
+#pragma unroll
+            for (int h = 0; h < SETS; ++h) {
+              const int at = (j * 2 + (GATED ? h : half)) * 128;
+              w[h] = src[at];
+              power[h] = src[powers - scales + at];
+            }
+            step(w, std::true_type(), power);
+          }
+          taken();
+          continue;
+        }
+        if constexpr (!GATED) {
+#pragma unroll
+          for (int j = 0; j < PW_BATCH; ++j) take(j);
+          taken();
+        }
+#pragma unroll
+        for (int j = 0; j < PW_BATCH; ++j) {
+          if (kq + j >= kblocks || err_code) continue;
+          if constexpr (GATED) take(j);
+          step(f[j % AHEAD], std::false_type(), nullptr);
         }
         if constexpr (GATED) taken();
       }
@@ -434,7 +481,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1) block_product_wide_kernel(const
 
 template <bool GATED>
 cudaError_t launch(PtParams &p, int64_t most_tiles, int num_sms, cudaStream_t s) {
-  const size_t misc = PT_EPI_WARPS * PW_STAGE_OUT + 8 * 8 + 16 + 2 * PW_SCALES * 4 + (3 * (size_t)p.groups + 1) * 4;
+  const size_t misc = PT_EPI_WARPS * PW_STAGE_OUT + 8 * 8 + 16 + 2 * PW_SLOT + (3 * (size_t)p.groups + 1) * 4;
   const size_t stage = (PW_ROWS + PW_WEIGHTS) * 128 + 16;
   p.stages = (int)((TC_SMEM_LIMIT - misc) / stage);
   // the attribute is the device's: set for each once

@@ -1,5 +1,6 @@
 """Every form that the products have, for each kind of operands: the counters say that the call took it."""
 import itertools
+import math
 
 import pytest
 import torch
@@ -132,3 +133,80 @@ def test_1100_rows_of_one_group(gated, n, indexed, tile):
     assert p(out, act) == 0
     assert [f for f, v in rt.form_counters().items() if v != before[f]] == [f"product_{tile}"]
     p.check(out, act)
+
+
+@pytest.mark.parametrize("case", [c for c in CASES if c[0] == "e4m3"], ids=lambda c: "-".join(map(str, c[1:])))
+def test_scales_whose_product_fp32_does_not_hold(case):
+    """Blocks of K in turn with weights' scales of about 1, 2^-75 and 2^64; rows of six kinds:
+    0  scales that make up for those
+    1  2^-75 where the weights have it: the product is 2^-150, the result about 2^-130; nothing elsewhere
+    2  2^64 where the weights have it and 2^-9 once there: the product is 2^128, the result up to 2^127; nothing elsewhere
+    3  2^64 where the weights have it, on zeros
+    4  nothing, with the smallest scale that quantising gives
+    5  of both signs: kinds 0 and 1 in one row, whose small blocks vanish beside the others
+    Gated: the gate is about 1/2, what it multiplies is as above."""
+    _, gated, indexed, tile, shares, rows, groups, n, k = case
+    p = Problem("e4m3", gated, indexed, rows, groups, n, k, 7 + CASES.index(case))
+    gen = generator(k)
+    blocks = ec.blocks(k)
+    e = torch.tensor([0, -75, 64], device="cuda").repeat(blocks)[:blocks]
+    p.sb = 0.25 + 0.25 * torch.rand(p.sb.shape, generator=gen, device="cuda")
+    if gated:
+        p.sb[:, 0] *= torch.exp2(torch.where(e == 64, -64, 0).float())
+        p.sb[:, 1] *= torch.exp2(e.float())
+        p.bias = torch.zeros(groups, 2, n, device="cuda")
+        p.bias[:, 0] = 0.5
+    else:
+        p.sb *= torch.exp2(e.float())
+        p.bias = None
+    kind = torch.arange(p.a.shape[0], device="cuda") % 6
+    if blocks < 3:
+        kind[kind == 2] = 0
+    of_kind = torch.stack([-e, torch.where(e == -75, -75, -64), torch.where(e == 64, 64, 0), torch.where(e == 64, 64, -64),
+                           torch.full_like(e, -126), torch.where(e == 64, -64, e)])[kind]
+    p.sa = torch.exp2(of_kind.float())
+    p.sa[kind == 5] *= -1
+    along = e.repeat_interleave(128)[:k]
+    a = p.a.float()
+    a[(kind == 1)[:, None] & (along != -75)] = 0
+    a[(kind == 2)[:, None].expand_as(a)] = 0
+    if blocks >= 3:
+        a[kind == 2, 2 * 128 + 5] = 2.0 ** -9
+    a[(kind == 3)[:, None] & (along == 64)] = 0
+    a[(kind == 4)[:, None].expand_as(a)] = 0
+    p.a = ec.rows_apart(a.to(torch.float8_e4m3fn).view(torch.uint8), 16).view(torch.float8_e4m3fn)
+    act = "gated" if gated else "none"
+    out = torch.full((rows, n), KEEP, device="cuda")
+    before = rt.form_counters()
+    assert p(out, act) == 0
+    assert [f for f, v in rt.form_counters().items() if v != before[f]] == [f"product_{tile}"]
+    p.check(out, act)
+    again = torch.empty_like(out)
+    assert p(again, act) == 0
+    assert torch.equal(out, again)
+
+
+def test_scales_that_are_no_numbers_or_zero():
+    """They act as the formula has it: zero takes its block away, an infinity or NaN makes the sums that it is in NaN or infinite."""
+    gen = generator(1)
+    (a, sa), (b, sb) = ec.e4m3(gen, 70, 640), ec.e4m3(gen, 200, 640, block_rows=128)
+    sa[3, 1], sa[9] = 0.0, 0.0
+    sa[20, 2], sa[21, 4], sa[22, 0] = math.inf, math.nan, 2.0 ** -149
+    out = torch.empty(70, 200, device="cuda")
+    assert ec.matmul(a, sa, b, sb, out) == 0
+    good = [r for r in range(70) if r not in (20, 21)]
+    want, slack = ec.product64(ec.values(a, sa, 1), ec.values(b, sb, 128), None, "none", torch.float32)
+    ec.close(out[good], want[good], slack[good])
+    assert not torch.isfinite(out[[20, 21]]).any() and torch.isnan(out[21]).all()
+
+
+def test_the_smallest_scale():
+    """2^-126: a factor below it is a multiple of 2^-149, half a step off at most; a block's sum is below 2^25."""
+    gen = generator(2)
+    for m in (7, 50, 300, 2100):
+        (a, sa), (b, sb) = ec.e4m3(gen, m, 640), ec.e4m3(gen, 200, 640, block_rows=128)
+        sa[::3] = 2.0 ** -126
+        out = torch.empty(m, 200, device="cuda")
+        assert ec.matmul(a, sa, b, sb, out) == 0
+        want, slack = ec.product64(ec.values(a, sa, 1), ec.values(b, sb, 128), None, "none", torch.float32)
+        ec.close(out, want, slack + 5 * 2.0 ** -125)
