@@ -263,60 +263,93 @@ def _ok(code):
 
 def _expert_rows(rng, B, L, timed, wanted):
     """The 8-bit and grouped operators; timed only when named in `only` ("e4m3", "grouped", "route", "combine").  VGG-16's first
-    classifier layer at the given batch; an expert layer with 32 experts, 4 for each of 16 B tokens."""
+    classifier layer at the given batch; an expert layer with 32 experts, 4 for each of 16 B tokens, and one with 64 for one token of
+    each of 32 sequences.  Operands are random numbers: zeros take less power."""
     s = L.occamy_stream()
+    held = []
 
-    def bytes_(n, random=False):
-        if not random:
-            return rt.DeviceBuffer(n)
-        return rt.DeviceBuffer.from_numpy(rng.integers(0, 120, n, dtype=np.uint8))   # e4m3 numbers up to 240
+    def keep(buf):
+        held.append(buf)
+        return buf
+
+    def bytes_(n):
+        return keep(rt.DeviceBuffer(n))
+
+    def e4m3(n):
+        return keep(rt.DeviceBuffer.from_numpy(rng.integers(0, 120, n, dtype=np.uint8) | rng.integers(0, 2, n, dtype=np.uint8) << 7))
+
+    def bf16(n):   # (cut off, not rounded)
+        return keep(rt.DeviceBuffer.from_numpy((rng.standard_normal(n, dtype=np.float32).view(np.uint32) >> 16).astype(np.uint16)))
+
+    def fp32(n):
+        return keep(rt.DeviceBuffer.from_numpy(rng.standard_normal(n, dtype=np.float32)))
+
+    def scales(n):
+        return keep(rt.DeviceBuffer.from_numpy(rng.random(n, dtype=np.float32) * 0.02 + 0.01))
+
+    def release():
+        for buf in held:
+            buf.free()
+        held.clear()
 
     def on(*pieces):
         return any(any(t in p for p in pieces) for t in wanted)
     n, k = 4096, 25088
-    if on("quantise e4m3 weights", "e4m3"):
-        w, q, qs = _T((n, k), rng.standard_normal((n, k), dtype=np.float32)), bytes_(n * k), bytes_(n * k // 4096)
-        timed(f"quantise e4m3 weights [{n},{k}] fp32", 5 * n * k,
-              lambda: _ok(L.occamy_quantize_e4m3(w.ptr, rt.F32, n, k, k, None, n, 128, q.ptr, k, qs.ptr, s)))
-        w.buf.free(), q.free(), qs.free()
+    for name, code, make, size in (("fp32", rt.F32, fp32, 4), ("bf16", rt.BF16, bf16, 2)):
+        if on("quantise e4m3 weights", "e4m3"):
+            w, q, qs = make(n * k), bytes_(n * k), bytes_(n * k // 4096)
+            timed(f"quantise e4m3 weights [{n},{k}] {name}", (size + 1) * n * k,
+                  lambda: _ok(L.occamy_quantize_e4m3(w.ptr, code, n, k, k, None, n, 128, q.ptr, k, qs.ptr, s)))
+            release()
     if on("product e4m3", "e4m3"):
-        a, b, sa, sb = bytes_(B * k, True), bytes_(n * k, True), bytes_(B * k // 32), bytes_(n * k // 4096)
-        out = bytes_(2 * B * n)
+        a, b, sa, sb, out = e4m3(B * k), e4m3(n * k), scales(B * k // 128), scales(n * k // 16384), bytes_(2 * B * n)
         timed(f"product e4m3 [{B},{k}] x [{n},{k}] ({2e-9 * B * n * k:.1f} GFLOP)", (B + n) * k + 2 * B * n,
               lambda: _ok(L.occamy_matmul_e4m3(a.ptr, k, sa.ptr, b.ptr, k, sb.ptr, None, B, n, k, 1, out.ptr, rt.BF16, n, s)))
-        for t in (a, b, sa, sb, out):
-            t.free()
+        release()
     if not on("grouped e4m3", "grouped bf16", "route", "combine", "quantise e4m3 rows", "e4m3"):
         return
-    tokens, experts, c, hidden, inner = 16 * B, 32, 4, 2048, 1024
-    rows = tokens * c
-    logits = _T((tokens, experts), rng.standard_normal((tokens, experts), dtype=np.float32))
-    chosen, weights, position, order = (bytes_(4 * rows) for _ in range(4))
-    offsets, need = bytes_(4 * (experts + 1)), L.occamy_route_experts_workspace(tokens, experts, c)
-    work = bytes_(max(need, 4))
+    hidden, inner, c = 2048, 1024, 4
+    for tokens, experts in ((16 * B, 32), (32, 64)):
+        rows = tokens * c
+        logits = fp32(tokens * experts)
+        chosen, weights, position, order = (bytes_(4 * rows) for _ in range(4))
+        offsets, need = bytes_(4 * (experts + 1)), L.occamy_route_experts_workspace(tokens, experts, c)
+        work = bytes_(max(need, 4))
 
-    def route():
-        _ok(L.occamy_route_experts(logits.ptr, rt.F32, tokens, experts, experts, c, 1, chosen.ptr, weights.ptr, offsets.ptr,
-                                   order.ptr, position.ptr, work.ptr, need, s))
-    route()
-    timed(f"route [{tokens},{experts}], {c} each", 4 * tokens * experts + 16 * rows, route)
-    x, q, qs = bytes_(2 * tokens * hidden), bytes_(rows * hidden), bytes_(rows * hidden // 32)
-    timed(f"quantise e4m3 rows [{tokens},{hidden}] bf16 -> {rows}", 2 * tokens * hidden + rows * hidden,
-          lambda: _ok(L.occamy_quantize_e4m3(x.ptr, rt.BF16, tokens, hidden, hidden, order.ptr, rows, 1, q.ptr, hidden, qs.ptr, s)))
-    y = bytes_(2 * rows * inner)
-    for name, code, size in (("e4m3", rt.E4M3, 1), ("bf16", rt.BF16, 2)):
-        b, sb = bytes_(experts * 2 * inner * hidden * size), bytes_(experts * 2 * inner * hidden // 4096)
+        def route():
+            _ok(L.occamy_route_experts(logits.ptr, rt.F32, tokens, experts, experts, c, 1, chosen.ptr, weights.ptr, offsets.ptr,
+                                       order.ptr, position.ptr, work.ptr, need, s))
+        route()
+        timed(f"route [{tokens},{experts}], {c} each", 4 * tokens * experts + 16 * rows, route)
+        xs = {"bf16": bf16(tokens * hidden), "fp32": fp32(tokens * hidden)}
+        q, qs = e4m3(rows * hidden), scales(rows * hidden // 128)
+        for name, code, size in (("fp32", rt.F32, 4), ("bf16", rt.BF16, 2)):
+            timed(f"quantise e4m3 rows [{tokens},{hidden}] {name} -> {rows}", size * tokens * hidden + rows * hidden,
+                  lambda: _ok(L.occamy_quantize_e4m3(xs[name].ptr, code, tokens, hidden, hidden, order.ptr, rows, 1, q.ptr, hidden,
+                                                     qs.ptr, s)))
+        xr = bf16(rows * hidden)
+        y = bf16(rows * inner)
         flops = 4.0 * rows * inner * hidden
-        timed(f"grouped {name}, gated, {rows} rows, {experts} x [{inner},{hidden}] ({flops / 1e9:.1f} GFLOP)",
-              (rows + experts * 2 * inner) * hidden * size + 2 * rows * inner,
-              lambda: _ok(L.occamy_matmul_grouped(q.ptr if size == 1 else x.ptr, code, rows if size == 1 else tokens, hidden,
-                                                  qs.ptr, None if size == 1 else order.ptr, offsets.ptr, experts, b.ptr, hidden,
-                                                  sb.ptr, None, rows, inner, hidden, rt.ACT_GATED_SILU, y.ptr, rt.BF16, inner, s)))
-        b.free(), sb.free()
-    out = bytes_(2 * tokens * inner)
-    timed(f"combine [{rows},{inner}] bf16 -> {tokens}", 2 * (rows + tokens) * inner,
-          lambda: _ok(L.occamy_combine_experts(y.ptr, rt.BF16, rows, inner, position.ptr, weights.ptr, tokens, c, inner, out.ptr,
-                                               rt.BF16, inner, s)))
+        for name, code, make, size in (("e4m3", rt.E4M3, e4m3, 1), ("bf16", rt.BF16, bf16, 2)):
+            b, sb = make(experts * 2 * inner * hidden), scales(experts * 2 * inner * hidden // 16384)
+            # rows in the order of their experts; chosen by an index (e4m3: of as many rows, as they are quantised)
+            for indexed in (False, True):
+                a = q if size == 1 else xs["bf16"] if indexed else xr
+                a_rows = tokens if size == 2 and indexed else rows
+                index = order.ptr if size == 2 else position.ptr
+                timed(f"grouped {name}, gated, {rows} rows{' by an index' if indexed else ''}, {experts} x [{inner},{hidden}] "
+                      f"({flops / 1e9:.1f} GFLOP)", (a_rows + experts * 2 * inner) * hidden * size + 2 * rows * inner,
+                      lambda: _ok(L.occamy_matmul_grouped(a.ptr, code, a_rows, hidden, qs.ptr, index if indexed else None,
+                                                          offsets.ptr, experts, b.ptr, hidden, sb.ptr, None, rows, inner, hidden,
+                                                          rt.ACT_GATED_SILU, y.ptr, rt.BF16, inner, s)))
+            for t in (b, sb):
+                t.free()
+                held.remove(t)
+        out = bytes_(2 * tokens * inner)
+        timed(f"combine [{rows},{inner}] bf16 -> {tokens}", 2 * (rows + tokens) * inner,
+              lambda: _ok(L.occamy_combine_experts(y.ptr, rt.BF16, rows, inner, position.ptr, weights.ptr, tokens, c, inner, out.ptr,
+                                                   rt.BF16, inner, s)))
+        release()
 
 
 def _rest(h, rng, B, L, timed, depthwise, sel):
