@@ -278,10 +278,13 @@ int64_t occamy_noalloc_capacity(void);
  *     while `stream` is captured, and while occamy_stream() is.
  *   - results have the same bits from call to call; elements of a result's rows behind its columns, and rows
  *     that no group or index reaches, are left as they were.  Sums are held in fp32.
+ *   - host threads: these calls may come from several at a time, but no other entry point of this library may run on
+ *     one thread while one of these runs on another, whatever memory they are given (they share the runtime's records).
  *   - returns 0 (also for an empty problem, which launches nothing), a negative code with a line on stderr and nothing
- *     enqueued (-1 no usable device, -2 workspace too small, -3 argument out of range, -5 a pointer that is not memory of the
- *     current device, -6 as above), or a cudaError_t.  The products' kernels have bounded waits: one that ran out leaves garbage
- *     in the result and a code that occamy_synchronize() collects for occamy_last_error(). */
+ *     enqueued (-1 no usable device, -2 workspace too small, -3 argument out of range, -4 out of host memory, -5 a pointer
+ *     that is not memory of the current device, -6 as above), or a cudaError_t.  The products' kernels have bounded waits:
+ *     one that ran out leaves garbage in the result and a code that occamy_synchronize(), called when `stream` is done,
+ *     collects for occamy_last_error(). */
 
 /* q = e4m3(x / s), s = 2^e with the smallest e >= -126 that keeps max|x| of the block within 448 s.  x has type 0, 1 or 2.
  * blockRows 1: a block is 128 elements of a row, and row i of q is row index[i] of x (index null: row i, and rows == xRows);

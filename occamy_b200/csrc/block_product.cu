@@ -188,191 +188,191 @@ __global__ void __launch_bounds__(PT_THREADS, BN <= 64 ? 2 : 1) block_product_ke
   // which nothing is spilled), of two CTAs (256 x 40 + 256 x 88) = 512 x 64.  (Each at the head of its roles: behind a point where both
   // come together the compiler keeps to the smaller number.)
   if (warp < PT_EPI_WARP) {
-  if constexpr (BN <= 64) asm volatile("setmaxnreg.dec.sync.aligned.u32 40;");
-  else if constexpr (BN == 256) asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
-  else asm volatile("setmaxnreg.dec.sync.aligned.u32 48;");
-  if (warp == 0) {
-    // ------------------------------------------------------------ loads
-    TCT_DECL
-    int stage = 0;
-    uint32_t phase = 0;
-    for (int tile = tile0; tile < total && !err_code; tile += tstep) {
-      const PtTile tl = decode(tile);
-      const int boxes = indexed ? 0 : (tl.rows + PT_BOX - 1) / PT_BOX;
-      const uint32_t bytes = W_BYTES + (uint32_t)boxes * (PT_BOX * 128u);
-      for (int kb = k0; kb < k1; ++kb) {
-        if (!TCT_WAIT(0, mbar_wait_warp(empty_bar(stage), phase ^ 1u, abort_flag))) {
-          err_code = 1;
-          break;
-        }
-        const int k = kb * (SCALED ? 128 : 64);
-        expect_tx_warp(full_bar(stage), bytes);
-        if constexpr (GATED) load_5d_warp(sW + stage * W_BYTES, &p.tb, full_bar(stage), k, tl.n0 / 8, tl.g);
-        else load_2d_warp(sW + stage * W_BYTES, &p.tb, full_bar(stage), k, tl.g * p.N + tl.n0);
-        const uint32_t dst = sR + stage * R_BYTES;
-        for (int b = 0; b < boxes; ++b)
-          load_2d_warp(dst + b * (PT_BOX * 128u), &p.ta, full_bar(stage), k, tl.m0 + b * PT_BOX);
-        if (++stage == stages) {
-          stage = 0;
-          phase ^= 1u;
-        }
-      }
-    }
-    TCT_FLUSH(0)
-    // Nothing may be under way to this CTA's memory when it ends: no arrivals of the last MMAs, and after an error no copies
-    // (the flag that ends other waits is set by then; these have their own).
-    int unset = 0;
-    for (int s = 0; s < stages; ++s) {
-      const uint32_t last_use = s < stage ? phase : phase ^ 1u;
-      mbar_wait_warp(err_code ? full_bar(s) : empty_bar(s), last_use, err_code ? &unset : abort_flag);
-    }
-  } else if (warp == 1) {
-    // ------------------------------------------------------------ MMAs
-    TCT_DECL
-    int stage = 0, buf = 0;
-    uint32_t phase = 0, buf_phase = 0;
-    const uint64_t w0 = make_smem_desc(sW, 64), r0 = make_smem_desc(sR, 64);
-    const uint32_t hi = (uint32_t)(w0 >> 32), w_lo = (uint32_t)w0, r_lo = (uint32_t)r0;
-    for (int tile = tile0; tile < total && !err_code; tile += tstep) {
-      const PtTile tl = decode(tile);
-      const uint32_t idesc = p.idesc | ((uint32_t)((tl.rows + 15) / 16 * 2) << 17);
-      int in_chunk = 0;
-      for (int kb = k0; kb < k1; ++kb) {
-        if (in_chunk == 0 && !TCT_WAIT(0, mbar_wait_warp(tempty_bar(buf), buf_phase ^ 1u, abort_flag))) {
-          err_code = 2;
-          break;
-        }
-        if (!TCT_WAIT(1, mbar_wait_warp(full_bar(stage), phase, abort_flag))) {
-          err_code = 3;
-          break;
-        }
-        if (indexed) fence_async_smem();
-        tc_fence_after();
-        const uint32_t d = tmem + (uint32_t)(buf * BN);
-        const uint32_t a = w_lo + (uint32_t)stage * (W_BYTES >> 4), b = r_lo + (uint32_t)stage * (R_BYTES >> 4);
-#pragma unroll
-        for (int kk = 0; kk < 4; ++kk)
-          pt_mma<SCALED>(d, a + 2u * kk, hi, b + 2u * kk, hi, idesc, kk ? 1u : (uint32_t)(in_chunk != 0));
-        commit_warp(empty_bar(stage));
-        if (++stage == stages) {
-          stage = 0;
-          phase ^= 1u;
-        }
-        if (++in_chunk == PER || kb + 1 == k1) {
-          commit_warp(tfull_bar(buf));
-          in_chunk = 0;
-          if (++buf == bufs) {
-            buf = 0;
-            buf_phase ^= 1u;
-          }
-        }
-      }
-    }
-    TCT_FLUSH(1)
-  } else if (warp >= PT_GATHER_WARP) {
-    // ------------------------------------------------------------ rows chosen by an index
-    if constexpr (BN < 256) {
-      if (p.index)
-        err_code = pt_gather_role<BN, PT_GATHERERS>(p, tile0, total, tstep, k0, k1, sR, stages, warp - PT_GATHER_WARP, lane, abort_flag,
-                                                    decode, full_bar, empty_bar);
-    }
-  } else {
-    // ------------------------------------------------------------ scales
-    // sA * sB of every column, one k-step after another.
-    if constexpr (SCALED) {
+    if constexpr (BN <= 64) asm volatile("setmaxnreg.dec.sync.aligned.u32 40;");
+    else if constexpr (BN == 256) asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
+    else asm volatile("setmaxnreg.dec.sync.aligned.u32 48;");
+    if (warp == 0) {
+      // ------------------------------------------------------------ loads
       TCT_DECL
-      constexpr int MINE = BN <= 64 ? 1 : BN / 64;
-      const int t = threadIdx.x - 64;
-      int buf = 0;
-      uint32_t buf_phase = 0, applied = 0;   // (a phase for each buffer)
+      int stage = 0;
+      uint32_t phase = 0;
       for (int tile = tile0; tile < total && !err_code; tile += tstep) {
         const PtTile tl = decode(tile);
-        const float *sa[MINE];
-#pragma unroll
-        for (int i = 0; i < MINE; ++i) {
-          const int c = t + 64 * i;
-          const int r = c < tl.rows ? (p.index ? p.index[tl.m0 + c] : tl.m0 + c) : -1;
-          sa[i] = r >= 0 && r < p.a_rows ? p.scale_a + (int64_t)r * p.kblocks : nullptr;
-        }
-        const float *sb = p.scale_b + ((int64_t)tl.g * SETS * p.blocks_n + tl.n0 / SCALE_BLOCK) * p.kblocks;
-        const int64_t second = (int64_t)p.blocks_n * p.kblocks;
-        float va[MINE][4], vb[SETS][4];
-        auto fetch = [&](int kq) {   // 1 where there is none (the numbers of a row that an index does not give are zeros)
-#pragma unroll
-          for (int j = 0; j < 4; ++j) {
-#pragma unroll
-            for (int i = 0; i < MINE; ++i) va[i][j] = sa[i] && kq + j < k1 ? __ldg(sa[i] + kq + j) : 1.0f;
-#pragma unroll
-            for (int h = 0; h < SETS; ++h) vb[h][j] = kq + j < k1 ? __ldg(sb + h * second + kq + j) : 1.0f;
+        const int boxes = indexed ? 0 : (tl.rows + PT_BOX - 1) / PT_BOX;
+        const uint32_t bytes = W_BYTES + (uint32_t)boxes * (PT_BOX * 128u);
+        for (int kb = k0; kb < k1; ++kb) {
+          if (!TCT_WAIT(0, mbar_wait_warp(empty_bar(stage), phase ^ 1u, abort_flag))) {
+            err_code = 1;
+            break;
           }
-        };
-        fetch(k0);
-        for (int kq = k0; kq < k1 && !err_code; kq += 4) {
-          uint32_t range = 0;   // of these four
+          const int k = kb * (SCALED ? 128 : 64);
+          expect_tx_warp(full_bar(stage), bytes);
+          if constexpr (GATED) load_5d_warp(sW + stage * W_BYTES, &p.tb, full_bar(stage), k, tl.n0 / 8, tl.g);
+          else load_2d_warp(sW + stage * W_BYTES, &p.tb, full_bar(stage), k, tl.g * p.N + tl.n0);
+          const uint32_t dst = sR + stage * R_BYTES;
+          for (int b = 0; b < boxes; ++b)
+            load_2d_warp(dst + b * (PT_BOX * 128u), &p.ta, full_bar(stage), k, tl.m0 + b * PT_BOX);
+          if (++stage == stages) {
+            stage = 0;
+            phase ^= 1u;
+          }
+        }
+      }
+      TCT_FLUSH(0)
+      // Nothing may be under way to this CTA's memory when it ends: no arrivals of the last MMAs, and after an error no copies
+      // (the flag that ends other waits is set by then; these have their own).
+      int unset = 0;
+      for (int s = 0; s < stages; ++s) {
+        const uint32_t last_use = s < stage ? phase : phase ^ 1u;
+        mbar_wait_warp(err_code ? full_bar(s) : empty_bar(s), last_use, err_code ? &unset : abort_flag);
+      }
+    } else if (warp == 1) {
+      // ------------------------------------------------------------ MMAs
+      TCT_DECL
+      int stage = 0, buf = 0;
+      uint32_t phase = 0, buf_phase = 0;
+      const uint64_t w0 = make_smem_desc(sW, 64), r0 = make_smem_desc(sR, 64);
+      const uint32_t hi = (uint32_t)(w0 >> 32), w_lo = (uint32_t)w0, r_lo = (uint32_t)r0;
+      for (int tile = tile0; tile < total && !err_code; tile += tstep) {
+        const PtTile tl = decode(tile);
+        const uint32_t idesc = p.idesc | ((uint32_t)((tl.rows + 15) / 16 * 2) << 17);
+        int in_chunk = 0;
+        for (int kb = k0; kb < k1; ++kb) {
+          if (in_chunk == 0 && !TCT_WAIT(0, mbar_wait_warp(tempty_bar(buf), buf_phase ^ 1u, abort_flag))) {
+            err_code = 2;
+            break;
+          }
+          if (!TCT_WAIT(1, mbar_wait_warp(full_bar(stage), phase, abort_flag))) {
+            err_code = 3;
+            break;
+          }
+          if (indexed) fence_async_smem();
+          tc_fence_after();
+          const uint32_t d = tmem + (uint32_t)(buf * BN);
+          const uint32_t a = w_lo + (uint32_t)stage * (W_BYTES >> 4), b = r_lo + (uint32_t)stage * (R_BYTES >> 4);
 #pragma unroll
-          for (int j = 0; j < 4; ++j)
-#pragma unroll
-            for (int i = 0; i < MINE; ++i)
-#pragma unroll
-              for (int h = 0; h < SETS; ++h) range = max(range, pt_range(va[i][j], vb[h][j]));
-          const bool look = __any_sync(0xffffffffu, range > PT_RANGE);
-#pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            if (kq + j >= k1 || err_code) continue;
-            if (!TCT_WAIT(0, mbar_wait_warp(tempty_bar(buf), buf_phase ^ 1u, abort_flag))) {
-              err_code = 4;
-              continue;
-            }
-            float *dst = scales + buf * (SETS * BN) + t;
-#pragma unroll
-            for (int i = 0; i < MINE; ++i)
-#pragma unroll
-              for (int h = 0; h < SETS; ++h)
-                if (BN >= 64 || t < BN) dst[h * BN + 64 * i] = va[i][j] * vb[h][j];
-            if (look) {
-              bool met = false;
-              float *pow = powers + buf * (SETS * BN) + t;
-#pragma unroll
-              for (int i = 0; i < MINE; ++i)
-#pragma unroll
-                for (int h = 0; h < SETS; ++h) {
-                  float f;
-                  const float power = pt_factor(va[i][j], vb[h][j], f);
-                  met = met || power != 1.0f;
-                  if (BN >= 64 || t < BN) dst[h * BN + 64 * i] = f, pow[h * BN + 64 * i] = power;
-                }
-              if (__any_sync(0xffffffffu, met)) {
-                // The sums' warps find this while they wait for the scales, which do not arrive before it is done; their loop does not look
-                // for it.  (A word read in every k-step took 256 x 4096 x 25088 from 50 us to 52 at best, 60 at worst.)
-                __threadfence_block();
-                __syncwarp();
-                if (lane == 0) wanted[2 * buf + warp - 2] = 1;
-                if (!mbar_wait_warp(applied_bar(buf, warp - 2), applied >> buf & 1u, abort_flag)) {
-                  err_code = 6;
-                  continue;
-                }
-                applied ^= 1u << buf;
-                if (lane == 0) wanted[2 * buf + warp - 2] = 0;
-              }
-            }
-            __syncwarp();
-            if (lane == 0) mbar_arrive(sfull_bar(buf));
+          for (int kk = 0; kk < 4; ++kk)
+            pt_mma<SCALED>(d, a + 2u * kk, hi, b + 2u * kk, hi, idesc, kk ? 1u : (uint32_t)(in_chunk != 0));
+          commit_warp(empty_bar(stage));
+          if (++stage == stages) {
+            stage = 0;
+            phase ^= 1u;
+          }
+          if (++in_chunk == PER || kb + 1 == k1) {
+            commit_warp(tfull_bar(buf));
+            in_chunk = 0;
             if (++buf == bufs) {
               buf = 0;
               buf_phase ^= 1u;
             }
           }
-          if (kq + 4 < k1) fetch(kq + 4);
         }
       }
-      if (warp == 2) { TCT_FLUSH(2) }
+      TCT_FLUSH(1)
+    } else if (warp >= PT_GATHER_WARP) {
+      // ------------------------------------------------------------ rows chosen by an index
+      if constexpr (BN < 256) {
+        if (p.index)
+          err_code = pt_gather_role<BN, PT_GATHERERS>(p, tile0, total, tstep, k0, k1, sR, stages, warp - PT_GATHER_WARP, lane, abort_flag,
+                                                      decode, full_bar, empty_bar);
+      }
+    } else {
+      // ------------------------------------------------------------ scales
+      // sA * sB of every column, one k-step after another.
+      if constexpr (SCALED) {
+        TCT_DECL
+        constexpr int MINE = BN <= 64 ? 1 : BN / 64;
+        const int t = threadIdx.x - 64;
+        int buf = 0;
+        uint32_t buf_phase = 0, applied = 0;   // (a phase for each buffer)
+        for (int tile = tile0; tile < total && !err_code; tile += tstep) {
+          const PtTile tl = decode(tile);
+          const float *sa[MINE];
+#pragma unroll
+          for (int i = 0; i < MINE; ++i) {
+            const int c = t + 64 * i;
+            const int r = c < tl.rows ? (p.index ? p.index[tl.m0 + c] : tl.m0 + c) : -1;
+            sa[i] = r >= 0 && r < p.a_rows ? p.scale_a + (int64_t)r * p.kblocks : nullptr;
+          }
+          const float *sb = p.scale_b + ((int64_t)tl.g * SETS * p.blocks_n + tl.n0 / SCALE_BLOCK) * p.kblocks;
+          const int64_t second = (int64_t)p.blocks_n * p.kblocks;
+          float va[MINE][4], vb[SETS][4];
+          auto fetch = [&](int kq) {   // 1 where there is none (the numbers of a row that an index does not give are zeros)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+#pragma unroll
+              for (int i = 0; i < MINE; ++i) va[i][j] = sa[i] && kq + j < k1 ? __ldg(sa[i] + kq + j) : 1.0f;
+#pragma unroll
+              for (int h = 0; h < SETS; ++h) vb[h][j] = kq + j < k1 ? __ldg(sb + h * second + kq + j) : 1.0f;
+            }
+          };
+          fetch(k0);
+          for (int kq = k0; kq < k1 && !err_code; kq += 4) {
+            uint32_t range = 0;   // of these four
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+#pragma unroll
+              for (int i = 0; i < MINE; ++i)
+#pragma unroll
+                for (int h = 0; h < SETS; ++h) range = max(range, pt_range(va[i][j], vb[h][j]));
+            const bool look = __any_sync(0xffffffffu, range > PT_RANGE);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+              if (kq + j >= k1 || err_code) continue;
+              if (!TCT_WAIT(0, mbar_wait_warp(tempty_bar(buf), buf_phase ^ 1u, abort_flag))) {
+                err_code = 4;
+                continue;
+              }
+              float *dst = scales + buf * (SETS * BN) + t;
+#pragma unroll
+              for (int i = 0; i < MINE; ++i)
+#pragma unroll
+                for (int h = 0; h < SETS; ++h)
+                  if (BN >= 64 || t < BN) dst[h * BN + 64 * i] = va[i][j] * vb[h][j];
+              if (look) {
+                bool met = false;
+                float *pow = powers + buf * (SETS * BN) + t;
+#pragma unroll
+                for (int i = 0; i < MINE; ++i)
+#pragma unroll
+                  for (int h = 0; h < SETS; ++h) {
+                    float f;
+                    const float power = pt_factor(va[i][j], vb[h][j], f);
+                    met = met || power != 1.0f;
+                    if (BN >= 64 || t < BN) dst[h * BN + 64 * i] = f, pow[h * BN + 64 * i] = power;
+                  }
+                if (__any_sync(0xffffffffu, met)) {
+                  // The sums' warps find this while they wait for the scales, which do not arrive before it is done; their loop does not look
+                  // for it.  (A word read in every k-step took 256 x 4096 x 25088 from 50 us to 52 at best, 60 at worst.)
+                  __threadfence_block();
+                  __syncwarp();
+                  if (lane == 0) wanted[2 * buf + warp - 2] = 1;
+                  if (!mbar_wait_warp(applied_bar(buf, warp - 2), applied >> buf & 1u, abort_flag)) {
+                    err_code = 6;
+                    continue;
+                  }
+                  applied ^= 1u << buf;
+                  if (lane == 0) wanted[2 * buf + warp - 2] = 0;
+                }
+              }
+              __syncwarp();
+              if (lane == 0) mbar_arrive(sfull_bar(buf));
+              if (++buf == bufs) {
+                buf = 0;
+                buf_phase ^= 1u;
+              }
+            }
+            if (kq + 4 < k1) fetch(kq + 4);
+          }
+        }
+        if (warp == 2) { TCT_FLUSH(2) }
+      }
     }
-  }
-  if (splits > 1) {   // where the sums' warps meet, the CTAs of the cluster among them
-    __syncwarp();
-    free_tmem();
-    cluster_sync_all();
-  }
+    if (splits > 1) {   // where the sums' warps meet, the CTAs of the cluster among them
+      __syncwarp();
+      free_tmem();
+      cluster_sync_all();
+    }
   } else {
     // ------------------------------------------------------------ sums and results
     if constexpr (BN <= 64) asm volatile("setmaxnreg.inc.sync.aligned.u32 88;");
@@ -622,7 +622,7 @@ int tile_height(const ProductArgs &a, int tiles_n, int num_sms) {
 // bf16, 32, 64, 128 and 256 in e4m3: 4096 rows, N = 1000, K = 4096 63 45 32 and 60 46 37 25; 300 rows 15 15 19 and 15 14 14 22; 2000 rows
 // in eight groups 37 29 31 and 34 26 36 24; 5000 in 32 89 74 66 and 76 64 60 48.)  Rows chosen by an index are copied at 18 bytes a
 // cycle of an SM, whatever the form: 16-bit tiles of 256 rows would wait for them and do without an index (16384 rows in 32 groups, gated,
-// 1024 x 2048 bf16: 32, 64 and 256 rows 259 199 264; without an index 266 172 144).
+// 1024 x 2048 bf16: 32, 64 and 256 rows 259 199 264; without an index 266 172 144; later 195 and 141 for what is taken).
 int choose_rows(const ProductArgs &a, bool scaled, bool gated, int kblocks, int num_sms) {
 #ifdef OCCAMY_TUNING
   if (const char *e = getenv("OCCAMY_PT_BN")) return !scaled && a.index ? std::min(atoi(e), 64) : atoi(e);

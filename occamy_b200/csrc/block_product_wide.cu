@@ -5,8 +5,9 @@
 // operands, copies and scales together.  A thread holds 128 sums of its row.  For each k-step it waits for the TMEM buffer, reads
 // 16 columns at a time and adds them, scaled.  On an SM that is 256 cycles of fp32 arithmetic and 150 of TMEM reads against the 512
 // that the tensor core takes for the k-step, but all eight warps go through it together, from one TMEM buffer's barrier to the
-// next, and with what they wait on the way a k-step takes them 950: that is what bounds the kernel (8190 x 8192 x 4096: 271 us, 2.0
-// PFLOP/s; without the sums 250, without the TMEM reads 254, without both 224, and of that the loads alone take 167, 19 TB/s out of L2).
+// next, and with what they wait on the way a k-step takes them 950: that is what bounds the kernel (8190 x 8192 x 4096: 275 us, 2.0
+// PFLOP/s.  Before it looked for factors out of range 271; then, without the sums 250, without the TMEM reads 254, without both 224, and of
+// that the loads alone took 167, 19 TB/s out of L2).
 // Tried: sixteen warps of 64 columns (310: no registers for their loads), loads of 32 or 64 columns (spills), either half of the weights
 // committed by itself (291 against 280 then), pairs of CTAs (cta_group::2, 288 to 330: less to load, but the second CTA's sums hold up
 // both).
@@ -96,163 +97,163 @@ __global__ void __launch_bounds__(PT_THREADS, 1) block_product_wide_kernel(const
   // The sums' warps take the registers that the others do without: 256 x 48 + 256 x 208 = 512 x 128.  (Each at the head of its
   // roles: behind a point where both come together the compiler keeps to the smaller number.)
   if (warp < PT_EPI_WARP) {
-  asm volatile("setmaxnreg.dec.sync.aligned.u32 48;");
-  if (warp == 0) {
-    // ------------------------------------------------------------ loads
-    TCT_DECL
-    int stage = 0;
-    uint32_t phase = 0;
-    for (int tile = tile0; tile < total && !err_code; tile += tstep) {
-      const PtTile tl = decode(tile);
-      const int boxes = p.index ? 0 : (tl.rows + PT_BOX - 1) / PT_BOX;
-      for (int kb = 0; kb < kblocks; ++kb) {
-        if (!TCT_WAIT(0, mbar_wait_warp(empty_bar(stage), phase ^ 1u, abort_flag))) {
-          err_code = 1;
-          break;
-        }
-        const int k = kb * 128;
-        expect_tx_warp(full_bar(stage), B_BYTES + (uint32_t)boxes * (PT_BOX * 128u));
-        if constexpr (GATED) load_5d_warp(sB + stage * B_BYTES, &p.tb, full_bar(stage), k, tl.n0 / 8, tl.g);
-        else load_2d_warp(sB + stage * B_BYTES, &p.tb, full_bar(stage), k, tl.g * p.N + tl.n0);
-        for (int b = 0; b < boxes; ++b)
-          load_2d_warp(sA + stage * A_BYTES + b * (PT_BOX * 128u), &p.ta, full_bar(stage), k, tl.m0 + b * PT_BOX);
-        if (++stage == stages) {
-          stage = 0;
-          phase ^= 1u;
-        }
-      }
-    }
-    TCT_FLUSH(0)
-    // Nothing may be under way to this CTA's memory when it ends: no arrivals of the last MMAs, and after an error no copies
-    // (the flag that ends other waits is set by then; these have their own).
-    int unset = 0;
-    for (int s = 0; s < stages; ++s) {
-      const uint32_t last_use = s < stage ? phase : phase ^ 1u;
-      mbar_wait_warp(err_code ? full_bar(s) : empty_bar(s), last_use, err_code ? &unset : abort_flag);
-    }
-  } else if (warp == 1) {
-    // ------------------------------------------------------------ MMAs
-    TCT_DECL
-    int stage = 0, buf = 0;
-    uint32_t phase = 0, buf_phase = 0;
-    const uint64_t a0 = make_smem_desc(sA, 64), b0 = make_smem_desc(sB, 64);
-    const uint32_t hi = (uint32_t)(a0 >> 32), a_lo = (uint32_t)a0, b_lo = (uint32_t)b0;
-    for (int tile = tile0; tile < total && !err_code; tile += tstep) {
-      const PtTile tl = decode(tile);
-      const int n = min(PW_WEIGHTS, ((p.N - tl.n0) * SETS + 15) / 16 * 16);   // no more weights than there are
-      const uint32_t idesc = p.idesc | ((uint32_t)(n >> 3) << 17);
-      for (int kb = 0; kb < kblocks; ++kb) {
-        if (!TCT_WAIT(0, mbar_wait_warp(tempty_bar(buf), buf_phase ^ 1u, abort_flag))) {
-          err_code = 2;
-          break;
-        }
-        if (!TCT_WAIT(1, mbar_wait_warp(full_bar(stage), phase, abort_flag))) {
-          err_code = 3;
-          break;
-        }
-        if (p.index) fence_async_smem();
-        tc_fence_after();
-        const uint32_t d = tmem + (uint32_t)(buf * PW_WEIGHTS);
-        const uint32_t a = a_lo + (uint32_t)stage * (A_BYTES >> 4), b = b_lo + (uint32_t)stage * (B_BYTES >> 4);
-#pragma unroll
-        for (int kk = 0; kk < 4; ++kk) pt_mma<true>(d, a + 2u * kk, hi, b + 2u * kk, hi, idesc, kk ? 1u : 0u);
-        commit_warp(empty_bar(stage));
-        commit_warp(tfull_bar(buf));
-        if (++stage == stages) {
-          stage = 0;
-          phase ^= 1u;
-        }
-        if (++buf == 2) {
-          buf = 0;
-          buf_phase ^= 1u;
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 48;");
+    if (warp == 0) {
+      // ------------------------------------------------------------ loads
+      TCT_DECL
+      int stage = 0;
+      uint32_t phase = 0;
+      for (int tile = tile0; tile < total && !err_code; tile += tstep) {
+        const PtTile tl = decode(tile);
+        const int boxes = p.index ? 0 : (tl.rows + PT_BOX - 1) / PT_BOX;
+        for (int kb = 0; kb < kblocks; ++kb) {
+          if (!TCT_WAIT(0, mbar_wait_warp(empty_bar(stage), phase ^ 1u, abort_flag))) {
+            err_code = 1;
+            break;
+          }
+          const int k = kb * 128;
+          expect_tx_warp(full_bar(stage), B_BYTES + (uint32_t)boxes * (PT_BOX * 128u));
+          if constexpr (GATED) load_5d_warp(sB + stage * B_BYTES, &p.tb, full_bar(stage), k, tl.n0 / 8, tl.g);
+          else load_2d_warp(sB + stage * B_BYTES, &p.tb, full_bar(stage), k, tl.g * p.N + tl.n0);
+          for (int b = 0; b < boxes; ++b)
+            load_2d_warp(sA + stage * A_BYTES + b * (PT_BOX * 128u), &p.ta, full_bar(stage), k, tl.m0 + b * PT_BOX);
+          if (++stage == stages) {
+            stage = 0;
+            phase ^= 1u;
+          }
         }
       }
-    }
-    TCT_FLUSH(1)
-  } else if (warp >= PT_GATHER_WARP) {
-    // ------------------------------------------------------------ rows chosen by an index
-    if (p.index)
-      err_code = pt_gather_role<PW_ROWS, PT_GATHERERS>(p, tile0, total, tstep, 0, kblocks, sA, stages, warp - PT_GATHER_WARP, lane,
-                                                       abort_flag, decode, full_bar, empty_bar);
-  } else {
-    // ------------------------------------------------------------ scales
-    // sA * sB of every row, with the scale of either half of the tile's weights (gated: of either matrix).
-    TCT_DECL
-    const int t = threadIdx.x - 64;
-    int slot = 0;
-    uint32_t slot_phase = 0;
-    for (int tile = tile0; tile < total && !err_code; tile += tstep) {
-      const PtTile tl = decode(tile);
-      const float *sa[2], *sb[2];
-#pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        const int m = t + 64 * i, r = m < tl.rows ? (p.index ? p.index[tl.m0 + m] : tl.m0 + m) : -1;
-        sa[i] = r >= 0 && r < p.a_rows ? p.scale_a + (int64_t)r * kblocks : nullptr;
+      TCT_FLUSH(0)
+      // Nothing may be under way to this CTA's memory when it ends: no arrivals of the last MMAs, and after an error no copies
+      // (the flag that ends other waits is set by then; these have their own).
+      int unset = 0;
+      for (int s = 0; s < stages; ++s) {
+        const uint32_t last_use = s < stage ? phase : phase ^ 1u;
+        mbar_wait_warp(err_code ? full_bar(s) : empty_bar(s), last_use, err_code ? &unset : abort_flag);
       }
+    } else if (warp == 1) {
+      // ------------------------------------------------------------ MMAs
+      TCT_DECL
+      int stage = 0, buf = 0;
+      uint32_t phase = 0, buf_phase = 0;
+      const uint64_t a0 = make_smem_desc(sA, 64), b0 = make_smem_desc(sB, 64);
+      const uint32_t hi = (uint32_t)(a0 >> 32), a_lo = (uint32_t)a0, b_lo = (uint32_t)b0;
+      for (int tile = tile0; tile < total && !err_code; tile += tstep) {
+        const PtTile tl = decode(tile);
+        const int n = min(PW_WEIGHTS, ((p.N - tl.n0) * SETS + 15) / 16 * 16);   // no more weights than there are
+        const uint32_t idesc = p.idesc | ((uint32_t)(n >> 3) << 17);
+        for (int kb = 0; kb < kblocks; ++kb) {
+          if (!TCT_WAIT(0, mbar_wait_warp(tempty_bar(buf), buf_phase ^ 1u, abort_flag))) {
+            err_code = 2;
+            break;
+          }
+          if (!TCT_WAIT(1, mbar_wait_warp(full_bar(stage), phase, abort_flag))) {
+            err_code = 3;
+            break;
+          }
+          if (p.index) fence_async_smem();
+          tc_fence_after();
+          const uint32_t d = tmem + (uint32_t)(buf * PW_WEIGHTS);
+          const uint32_t a = a_lo + (uint32_t)stage * (A_BYTES >> 4), b = b_lo + (uint32_t)stage * (B_BYTES >> 4);
 #pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        const int block = GATED ? h * p.blocks_n + tl.n0 / SCALE_BLOCK : min(tl.n0 / SCALE_BLOCK + h, p.blocks_n - 1);
-        sb[h] = p.scale_b + ((int64_t)tl.g * SETS * p.blocks_n + block) * kblocks;
+          for (int kk = 0; kk < 4; ++kk) pt_mma<true>(d, a + 2u * kk, hi, b + 2u * kk, hi, idesc, kk ? 1u : 0u);
+          commit_warp(empty_bar(stage));
+          commit_warp(tfull_bar(buf));
+          if (++stage == stages) {
+            stage = 0;
+            phase ^= 1u;
+          }
+          if (++buf == 2) {
+            buf = 0;
+            buf_phase ^= 1u;
+          }
+        }
       }
-      float va[2][PW_BATCH], vb[2][PW_BATCH];
-      auto fetch = [&](int kq) {   // 1 where there is none (the numbers of a row that an index does not give are zeros)
+      TCT_FLUSH(1)
+    } else if (warp >= PT_GATHER_WARP) {
+      // ------------------------------------------------------------ rows chosen by an index
+      if (p.index)
+        err_code = pt_gather_role<PW_ROWS, PT_GATHERERS>(p, tile0, total, tstep, 0, kblocks, sA, stages, warp - PT_GATHER_WARP, lane,
+                                                         abort_flag, decode, full_bar, empty_bar);
+    } else {
+      // ------------------------------------------------------------ scales
+      // sA * sB of every row, with the scale of either half of the tile's weights (gated: of either matrix).
+      TCT_DECL
+      const int t = threadIdx.x - 64;
+      int slot = 0;
+      uint32_t slot_phase = 0;
+      for (int tile = tile0; tile < total && !err_code; tile += tstep) {
+        const PtTile tl = decode(tile);
+        const float *sa[2], *sb[2];
 #pragma unroll
-        for (int j = 0; j < PW_BATCH; ++j) {
-#pragma unroll
-          for (int i = 0; i < 2; ++i) va[i][j] = sa[i] && kq + j < kblocks ? __ldg(sa[i] + kq + j) : 1.0f;
-#pragma unroll
-          for (int h = 0; h < 2; ++h) vb[h][j] = kq + j < kblocks ? __ldg(sb[h] + kq + j) : 1.0f;
+        for (int i = 0; i < 2; ++i) {
+          const int m = t + 64 * i, r = m < tl.rows ? (p.index ? p.index[tl.m0 + m] : tl.m0 + m) : -1;
+          sa[i] = r >= 0 && r < p.a_rows ? p.scale_a + (int64_t)r * kblocks : nullptr;
         }
-      };
-      fetch(0);
-      for (int kq = 0; kq < kblocks; kq += PW_BATCH) {
-        uint32_t range = 0;
 #pragma unroll
-        for (int j = 0; j < PW_BATCH; ++j)
-#pragma unroll
-          for (int h = 0; h < 2; ++h)
-#pragma unroll
-            for (int i = 0; i < 2; ++i) range = max(range, pt_range(va[i][j], vb[h][j]));
-        const bool look = __any_sync(0xffffffffu, range > PT_RANGE);
-        if (!TCT_WAIT(0, mbar_wait_warp(sempty_bar(slot), slot_phase ^ 1u, abort_flag))) {
-          err_code = 4;
-          break;
+        for (int h = 0; h < 2; ++h) {
+          const int block = GATED ? h * p.blocks_n + tl.n0 / SCALE_BLOCK : min(tl.n0 / SCALE_BLOCK + h, p.blocks_n - 1);
+          sb[h] = p.scale_b + ((int64_t)tl.g * SETS * p.blocks_n + block) * kblocks;
         }
-        float *dst = scales + slot * PW_SCALES + t;
+        float va[2][PW_BATCH], vb[2][PW_BATCH];
+        auto fetch = [&](int kq) {   // 1 where there is none (the numbers of a row that an index does not give are zeros)
 #pragma unroll
-        for (int j = 0; j < PW_BATCH; ++j)
+          for (int j = 0; j < PW_BATCH; ++j) {
 #pragma unroll
-          for (int h = 0; h < 2; ++h)
+            for (int i = 0; i < 2; ++i) va[i][j] = sa[i] && kq + j < kblocks ? __ldg(sa[i] + kq + j) : 1.0f;
 #pragma unroll
-            for (int i = 0; i < 2; ++i) dst[(j * 2 + h) * 128 + 64 * i] = va[i][j] * vb[h][j];
-        bool met = false;
-        if (look) {
-          float *pow = powers + slot * PW_SCALES + t;
+            for (int h = 0; h < 2; ++h) vb[h][j] = kq + j < kblocks ? __ldg(sb[h] + kq + j) : 1.0f;
+          }
+        };
+        fetch(0);
+        for (int kq = 0; kq < kblocks; kq += PW_BATCH) {
+          uint32_t range = 0;
 #pragma unroll
           for (int j = 0; j < PW_BATCH; ++j)
 #pragma unroll
             for (int h = 0; h < 2; ++h)
 #pragma unroll
-              for (int i = 0; i < 2; ++i) {
-                float f;
-                const float power = pt_factor(va[i][j], vb[h][j], f);
-                met = met || power != 1.0f;
-                dst[(j * 2 + h) * 128 + 64 * i] = f, pow[(j * 2 + h) * 128 + 64 * i] = power;
-              }
-          met = __any_sync(0xffffffffu, met);
+              for (int i = 0; i < 2; ++i) range = max(range, pt_range(va[i][j], vb[h][j]));
+          const bool look = __any_sync(0xffffffffu, range > PT_RANGE);
+          if (!TCT_WAIT(0, mbar_wait_warp(sempty_bar(slot), slot_phase ^ 1u, abort_flag))) {
+            err_code = 4;
+            break;
+          }
+          float *dst = scales + slot * PW_SCALES + t;
+#pragma unroll
+          for (int j = 0; j < PW_BATCH; ++j)
+#pragma unroll
+            for (int h = 0; h < 2; ++h)
+#pragma unroll
+              for (int i = 0; i < 2; ++i) dst[(j * 2 + h) * 128 + 64 * i] = va[i][j] * vb[h][j];
+          bool met = false;
+          if (look) {
+            float *pow = powers + slot * PW_SCALES + t;
+#pragma unroll
+            for (int j = 0; j < PW_BATCH; ++j)
+#pragma unroll
+              for (int h = 0; h < 2; ++h)
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {
+                  float f;
+                  const float power = pt_factor(va[i][j], vb[h][j], f);
+                  met = met || power != 1.0f;
+                  dst[(j * 2 + h) * 128 + 64 * i] = f, pow[(j * 2 + h) * 128 + 64 * i] = power;
+                }
+            met = __any_sync(0xffffffffu, met);
+          }
+          if (lane == 0) reinterpret_cast<uint32_t *>(any_power + slot)[warp - 2] = met;
+          __syncwarp();
+          if (lane == 0) mbar_arrive(sfull_bar(slot));
+          if (++slot == 2) {
+            slot = 0;
+            slot_phase ^= 1u;
+          }
+          if (kq + PW_BATCH < kblocks) fetch(kq + PW_BATCH);   // there when the next slot is free
         }
-        if (lane == 0) reinterpret_cast<uint32_t *>(any_power + slot)[warp - 2] = met;
-        __syncwarp();
-        if (lane == 0) mbar_arrive(sfull_bar(slot));
-        if (++slot == 2) {
-          slot = 0;
-          slot_phase ^= 1u;
-        }
-        if (kq + PW_BATCH < kblocks) fetch(kq + PW_BATCH);   // there when the next slot is free
       }
+      if (warp == 2) { TCT_FLUSH(2) }
     }
-    if (warp == 2) { TCT_FLUSH(2) }
-  }
   } else {
     // ------------------------------------------------------------ sums and results
     asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
@@ -262,7 +263,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1) block_product_wide_kernel(const
     uint32_t buf_phase = 0, slot_phase = 0;
     for (int tile = tile0; tile < total && !err_code; tile += tstep) {
       const PtTile tl = decode(tile);
-            float acc[PW_COLUMNS];   // from the bias on
+      float acc[PW_COLUMNS];   // from the bias on
 #pragma unroll
       for (int i = 0; i < PW_COLUMNS; ++i) acc[i] = 0.0f;
       const int n_tile = min(TILE_N, p.N - tl.n0);
